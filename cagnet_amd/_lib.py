@@ -6,7 +6,7 @@ the import of this module raises; nothing here computes on the CPU.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint32, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libcagnet_amd.so"
@@ -15,6 +15,9 @@ CG_OK = 0
 CG_CSR_SORTED = 1
 CG_CSR_TRANSPOSE = 2
 CG_CSR_VALIDATE = 4
+
+CG_F32, CG_BF16, CG_F16 = 0, 1, 2
+CG_GATE_NONE, CG_GATE_ROW, CG_GATE_FULL = 0, 1, 2
 
 CG_ERR_UNSUPPORTED = 8
 STATUS_NAMES = {
@@ -71,6 +74,20 @@ _SIGNATURES = {
     "cg_nll_loss_bwd": [P, P, P, P, P, c_int64, c_int64, c_int32, P],
     "cg_log_softmax_nll_bwd": [P, c_int64, P, P, P, P, P, c_int64, c_int64, c_int32, P],
     "cg_log_softmax_nll_fwd": [P, c_int64, P, P, P, c_int64, c_int64, c_int32, P, P, P],
+    "cg_rng_next": [P, P, P],
+    "cg_dropout": [P, c_int64, P, c_int64, c_int64, c_int32, c_int, c_double, P, P],
+    "cg_embedding_fwd": [P, c_int64, c_int64, P, c_int, c_int64, c_int32, c_int, c_float, P, c_int64, P],
+    "cg_embedding_bwd_workspace": [c_int64, c_int64, c_int32, POINTER(c_int64)],
+    "cg_embedding_bwd": [P, c_int64, P, c_int, c_int64, c_int64, c_int32, c_int, c_int, c_float, c_float, P, c_int64, P,
+                         c_int64, P],
+    "cg_rms_norm_fwd": [P, c_int64, P, c_int, P, c_int64, P, c_int64, c_int32, c_int, c_float, P],
+    "cg_norm_bwd_workspace": [c_int64, c_int32, POINTER(c_int64)],
+    "cg_rms_norm_bwd": [P, c_int64, P, c_int64, P, c_int, P, P, c_int64, P, c_int64, c_int32, c_int, P, c_int64, P],
+    "cg_norm_residual_fwd": [P, c_int64, P, c_int64, P, c_int64, c_int, P, P, P, c_int, c_float, c_double, P, c_float,
+                             P, c_int64, P, c_int64, P, P, c_int64, c_int32, c_int, P],
+    "cg_norm_residual_bwd": [P, c_int64, P, c_int64, P, c_int64, P, c_int64, P, c_int64, c_int, P, P, P, c_int, c_float,
+                             c_double, P, P, P, P, c_int64, P, c_int64, P, c_int64, P, P, P, c_int64, c_int32, c_int, P,
+                             c_int64, P],
     "cg_csr_blob_size": [P, POINTER(c_int64)],
     "cg_csr_blob_write": [P, P, c_int64, P],
     "cg_csr_blob_read": [POINTER(c_void_p), P, c_int64, c_uint32, P],

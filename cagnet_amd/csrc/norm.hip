@@ -1,0 +1,370 @@
+// Root-mean-square norms of rows, alone (rms_norm) and on both sides of a residual block (norm_residual):
+//   rms_norm       y = x rho w,                                        rho = 1 / sqrt(mean(x^2) + eps)
+//   norm_residual  u = alpha scale keep(sigmoid(gate) z rho_z w_post),  r = x + u,  h = r rho_r w_pre
+// and their gradients.  With t = g w and xh = x rho, dx = rho (t - xh mean(t xh)) and dw = sum over rows of g xh.
+// Statistics, sums and everything between a load and the one rounding at a store are float32.
+#include "rows.h"
+#include <limits.h>
+
+namespace cg {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormWaves = kNormThreads / kWave;
+
+// Arguments of either operator, forward and backward; rms_norm uses the z side as its input x and leaves the rest
+// at its defaults.
+struct NormArgs {
+  const void *z, *x, *gate, *dr, *dh, *r_in;
+  void *r, *h, *dz, *dx, *dgate;
+  int64_t ldz, ldx, ldgate, lddr, lddh, ldr_in, ldr, ldh, lddz, lddx, lddgate;
+  const void *w_post, *w_pre, *scale;
+  int w_f32, gate_kind;
+  float alpha, eps;
+  float *rstd_z, *rstd_r;  // written forward, read backward
+  float *partial;          // backward: [workgroups][2][d]: columns of q and of dw_pre
+  Mask mask;
+  int64_t n;
+  int32_t d;
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+// every thread of the workgroup gets the sum; `slots` is rewritten only after everybody has read it
+__device__ __forceinline__ float group_sum(float v, float *slots) {
+  v = wave_sum(v);
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  __syncthreads();
+  if (lane == 0) slots[wave] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) s += slots[w];
+  return s;
+}
+__device__ __forceinline__ float sigmoid(float a) { return 1.f / (1.f + expf(-a)); }
+
+// ---------------------------------------------------------------------------------------------
+// Rows of any length: one workgroup per row, the row read again for every pass over it.
+// ---------------------------------------------------------------------------------------------
+template <int DT, bool RESIDUAL>
+__global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a) {
+  typedef typename Elem<DT>::type T;
+  __shared__ float slots[kNormWaves];
+  MaskKey key = {0, 0, 0, 0};
+  if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T *z = (const T *)a.z + row * a.ldz;
+    float s = 0.f;
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) s += (float)z[j] * (float)z[j];
+    const float rho_z = 1.f / sqrtf(group_sum(s, slots) / (float)a.d + a.eps);
+    if (threadIdx.x == 0) a.rstd_z[row] = rho_z;
+    if (!RESIDUAL) {
+      T *h = (T *)a.h + row * a.ldh;
+      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
+        h[j] = (T)((float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j));
+      continue;
+    }
+    const T *x = (const T *)a.x + row * a.ldx;
+    const T *gate = a.gate_kind ? (const T *)a.gate + row * a.ldgate : nullptr;
+    auto sum_at = [&](int32_t j) {
+      float u = (float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j);
+      if (gate) u *= sigmoid((float)gate[a.gate_kind == CG_GATE_ROW ? 0 : j]);
+      if (a.mask.rng) u = mask_at(key, a.mask, row, j) > 0.f ? u * a.mask.inv_keep : 0.f;
+      return (float)x[j] + a.alpha * weight_at<T>(a.scale, a.w_f32, j) * u;
+    };
+    s = 0.f;
+    T *r = (T *)a.r + row * a.ldr, *h = (T *)a.h + row * a.ldh;
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
+      const float v = sum_at(j);
+      r[j] = (T)v;
+      s += v * v;
+    }
+    const float rho_r = 1.f / sqrtf(group_sum(s, slots) / (float)a.d + a.eps);
+    if (threadIdx.x == 0) a.rstd_r[row] = rho_r;
+    // h comes from the sum before its rounding to the stored type
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = (T)(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
+  }
+}
+
+// The gradients of the weights are sums over rows: every workgroup adds its rows up in its own slice of `partial`
+// (each column belongs to one thread), and a second kernel adds the slices in order.
+template <int DT, bool RESIDUAL>
+__global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a) {
+  typedef typename Elem<DT>::type T;
+  __shared__ float slots[kNormWaves];
+  MaskKey key = {0, 0, 0, 0};
+  if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
+  float *q = a.partial + (int64_t)blockIdx.x * 2 * a.d, *dwp = q + a.d;
+  for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) q[j] = dwp[j] = 0.f;
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+    const T *z = (const T *)a.z + row * a.ldz;
+    const T *dh = a.dh ? (const T *)a.dh + row * a.lddh : nullptr;
+    T *dz = (T *)a.dz + row * a.lddz;
+    const float rho_z = a.rstd_z[row];
+    if (!RESIDUAL) {
+      float s = 0.f;
+      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
+        s += (float)dh[j] * weight_at<T>(a.w_post, a.w_f32, j) * ((float)z[j] * rho_z);
+      const float m = group_sum(s, slots) / (float)a.d;
+      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
+        const float zh = (float)z[j] * rho_z, g = (float)dh[j];
+        q[j] += g * zh;
+        dz[j] = (T)(rho_z * (g * weight_at<T>(a.w_post, a.w_f32, j) - zh * m));
+      }
+      continue;
+    }
+    const T *r = (const T *)a.r_in + row * a.ldr_in;
+    const T *dr = a.dr ? (const T *)a.dr + row * a.lddr : nullptr;
+    const T *gate = a.gate_kind ? (const T *)a.gate + row * a.ldgate : nullptr;
+    const float rho_r = a.rstd_r[row];
+    float mean_r = 0.f;
+    if (dh) {
+      float s = 0.f;
+      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
+        s += (float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) * ((float)r[j] * rho_r);
+      mean_r = group_sum(s, slots) / (float)a.d;
+    }
+    auto into = [&](int32_t j) {  // gradient of the residual sum
+      float v = dr ? (float)dr[j] : 0.f;
+      if (dh) v += rho_r * ((float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) - (float)r[j] * rho_r * mean_r);
+      return v;
+    };
+    auto gate_at = [&](int32_t j) { return gate ? sigmoid((float)gate[a.gate_kind == CG_GATE_ROW ? 0 : j]) : 1.f; };
+    auto keep_at = [&](int32_t j) { return a.mask.rng ? mask_at(key, a.mask, row, j) : 1.f; };
+    float s = 0.f, sg = 0.f;
+    T *dx = (T *)a.dx + row * a.lddx;
+    T *dgate = a.dgate ? (T *)a.dgate + row * a.lddgate : nullptr;
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
+      const float D = into(j), zh = (float)z[j] * rho_z, sig = gate_at(j), Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
+      const float e = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j);
+      dx[j] = (T)D;
+      s += e * sig * zh;
+      q[j] += Dm * sig * zh;
+      if (dh) dwp[j] += (float)dh[j] * ((float)r[j] * rho_r);
+      const float dg = e * zh * (sig * (1.f - sig));
+      if (a.gate_kind == CG_GATE_ROW)
+        sg += dg;
+      else if (dgate)
+        dgate[j] = (T)dg;
+    }
+    const float mean_z = group_sum(s, slots) / (float)a.d;
+    if (a.gate_kind == CG_GATE_ROW) {
+      sg = group_sum(sg, slots);
+      if (dgate && threadIdx.x == 0) dgate[0] = (T)sg;
+    }
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
+      const float D = into(j), zh = (float)z[j] * rho_z, Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
+      const float f = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j) * gate_at(j);
+      dz[j] = (T)(rho_z * (f - zh * mean_z));
+    }
+  }
+}
+
+// dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added in order.  One workgroup per
+// 64 columns; its 4 waves take every fourth slice, then their four sums are added in order.
+template <int DT>
+__global__ __launch_bounds__(kNormThreads) void norm_weight_grads_kernel(NormArgs a, int32_t slices, void *dw_post,
+                                                                         void *dw_pre, void *dscale) {
+  typedef typename Elem<DT>::type T;
+  __shared__ float sq[kNormWaves][kWave], sp[kNormWaves][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int32_t j = blockIdx.x * kWave + lane;
+  float q = 0.f, p = 0.f;
+  if (j < a.d)
+    for (int32_t k = wave; k < slices; k += kNormWaves) {
+      const float *at = a.partial + (int64_t)k * 2 * a.d + j;
+      q += at[0];
+      p += at[a.d];
+    }
+  sq[wave][lane] = q;
+  sp[wave][lane] = p;
+  __syncthreads();
+  if (wave != 0 || j >= a.d) return;
+  q = p = 0.f;
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) {
+    q += sq[w][lane];
+    p += sp[w][lane];
+  }
+  if (dw_post) weight_put<T>(dw_post, a.w_f32, j, a.alpha * weight_at<T>(a.scale, a.w_f32, j) * q);
+  if (dscale) weight_put<T>(dscale, a.w_f32, j, a.alpha * weight_at<T>(a.w_post, a.w_f32, j) * q);
+  if (dw_pre) weight_put<T>(dw_pre, a.w_f32, j, p);
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+constexpr int64_t kNormMaxGroups = 1024;  // four workgroups per compute unit
+
+static int64_t norm_groups(int64_t n) { return n < kNormMaxGroups ? n : kNormMaxGroups; }
+
+static size_t norm_workspace(int64_t n, int32_t d) { return (size_t)norm_groups(n) * 2 * (size_t)d * sizeof(float); }
+
+static int check_weights(const char *who, int dtype, int wdtype) {
+  if (wdtype != CG_F32 && wdtype != dtype)
+    CG_FAIL(CG_ERR_UNSUPPORTED, "%s: weights of dtype %d beside activations of dtype %d (CG_F32 or the same)", who, wdtype, dtype);
+  return CG_OK;
+}
+static int check_float(const char *who, const char *what, float v, bool positive) {
+  if (!(v - v == 0.f) || (positive && !(v > 0.f)))
+    CG_FAIL(CG_ERR_SIZE, "%s: %s=%g has to be finite%s", who, what, (double)v, positive ? " and above zero" : "");
+  return CG_OK;
+}
+
+template <bool RESIDUAL>
+static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
+  int64_t groups = a.n < 256 * 32 ? a.n : 256 * 32;
+#define CG_CALL(DT) norm_fwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
+  CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_CALL
+  CG_LAUNCH_CHECK();
+  return CG_OK;
+}
+
+template <bool RESIDUAL>
+static int norm_bwd(const NormArgs &a, int dtype, void *dw_post, void *dw_pre, void *dscale, hipStream_t s) {
+  const int64_t groups = norm_groups(a.n);
+  if (groups > 0) {
+#define CG_CALL(DT) norm_bwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
+    CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_CALL
+    CG_LAUNCH_CHECK();
+  }
+  if (dw_post || dw_pre || dscale) {
+#define CG_CALL(DT)                                                                                                   \
+  norm_weight_grads_kernel<DT><<<(unsigned)ceil_div64(a.d, kWave), kNormThreads, 0, s>>>(a, (int32_t)groups, dw_post, \
+                                                                                         dw_pre, dscale)
+    CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_CALL
+    CG_LAUNCH_CHECK();
+  }
+  return CG_OK;
+}
+
+}  // namespace cg
+
+extern "C" {
+
+int cg_norm_bwd_workspace(int64_t n, int32_t d, int64_t *bytes) {
+  using namespace cg;
+  if (!bytes) CG_FAIL(CG_ERR_NULL, "cg_norm_bwd_workspace: null pointer");
+  CG_TRY(check_row_shape("cg_norm_bwd_workspace", n, d));
+  *bytes = (int64_t)norm_workspace(n, d);
+  return CG_OK;
+}
+
+int cg_rms_norm_fwd(const void *d_x, int64_t ldx, const void *d_w, int wdtype, void *d_y, int64_t ldy, float *d_rstd,
+                    int64_t n, int32_t d, int dtype, float eps, cg_stream_t stream) {
+  using namespace cg;
+  const char *who = "cg_rms_norm_fwd";
+  CG_TRY(check_dtype(who, dtype));
+  CG_TRY(check_weights(who, dtype, wdtype));
+  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_float(who, "eps", eps, true));
+  if (n == 0) return CG_OK;
+  if (!d_x || !d_y || !d_rstd) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
+  if (ldx < d || ldy < d) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
+  if (d_x == d_y) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the input", who);
+  NormArgs a = {};
+  a.z = d_x, a.ldz = ldx, a.w_post = d_w, a.w_f32 = wdtype == CG_F32, a.h = d_y, a.ldh = ldy, a.rstd_z = d_rstd;
+  a.n = n, a.d = d, a.eps = eps, a.alpha = 1.f;
+  ProfScope prof("rms_norm_fwd", d, (hipStream_t)stream);
+  return norm_fwd<false>(a, dtype, (hipStream_t)stream);
+}
+
+int cg_rms_norm_bwd(const void *d_g, int64_t ldg, const void *d_x, int64_t ldx, const void *d_w, int wdtype,
+                    const float *d_rstd, void *d_dx, int64_t lddx, void *d_dw, int64_t n, int32_t d, int dtype,
+                    void *d_work, int64_t work_bytes, cg_stream_t stream) {
+  using namespace cg;
+  const char *who = "cg_rms_norm_bwd";
+  CG_TRY(check_dtype(who, dtype));
+  CG_TRY(check_weights(who, dtype, wdtype));
+  CG_TRY(check_row_shape(who, n, d));
+  if (n > 0) {
+    if (!d_g || !d_x || !d_rstd || !d_dx || !d_work) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
+    if (ldg < d || ldx < d || lddx < d) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
+    if (d_dx == d_g || d_dx == d_x) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be an input", who);
+    if (work_bytes < (int64_t)norm_workspace(n, d)) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)norm_workspace(n, d));
+  }
+  NormArgs a = {};
+  a.dh = d_g, a.lddh = ldg, a.z = d_x, a.ldz = ldx, a.w_post = d_w, a.w_f32 = wdtype == CG_F32;
+  a.rstd_z = const_cast<float *>(d_rstd), a.dz = d_dx, a.lddz = lddx, a.partial = (float *)d_work;
+  a.n = n, a.d = d, a.alpha = 1.f;
+  ProfScope prof("rms_norm_bwd", d, (hipStream_t)stream);
+  return norm_bwd<false>(a, dtype, d_dw, nullptr, nullptr, (hipStream_t)stream);
+}
+
+int cg_norm_residual_fwd(const void *d_z, int64_t ldz, const void *d_x, int64_t ldx, const void *d_gate, int64_t ldgate,
+                         int gate_kind, const void *d_w_post, const void *d_w_pre, const void *d_scale, int wdtype,
+                         float alpha, double p, const int64_t *d_rng, float eps, void *d_r, int64_t ldr, void *d_h,
+                         int64_t ldh, float *d_rstd_z, float *d_rstd_r, int64_t n, int32_t d, int dtype,
+                         cg_stream_t stream) {
+  using namespace cg;
+  const char *who = "cg_norm_residual_fwd";
+  CG_TRY(check_dtype(who, dtype));
+  CG_TRY(check_weights(who, dtype, wdtype));
+  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_float(who, "eps", eps, true));
+  CG_TRY(check_float(who, "alpha", alpha, false));
+  CG_TRY(check_p(who, p, d_rng));
+  if (gate_kind < CG_GATE_NONE || gate_kind > CG_GATE_FULL) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: gate kind %d", who, gate_kind);
+  if (n == 0) return CG_OK;
+  if (!d_z || !d_x || !d_r || !d_h || !d_rstd_z || !d_rstd_r || (gate_kind != CG_GATE_NONE && !d_gate))
+    CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
+  if (ldz < d || ldx < d || ldr < d || ldh < d || (gate_kind == CG_GATE_FULL && ldgate < d) || (gate_kind == CG_GATE_ROW && ldgate < 1))
+    CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
+  if (d_r == d_z || d_r == d_x || d_h == d_z || d_h == d_x || d_r == d_h || (gate_kind != CG_GATE_NONE && (d_r == d_gate || d_h == d_gate)))
+    CG_FAIL(CG_ERR_ALIAS, "%s: an output may not be an input or the other output", who);
+  NormArgs a = {};
+  a.z = d_z, a.ldz = ldz, a.x = d_x, a.ldx = ldx, a.gate = d_gate, a.ldgate = ldgate, a.gate_kind = gate_kind;
+  a.w_post = d_w_post, a.w_pre = d_w_pre, a.scale = d_scale, a.w_f32 = wdtype == CG_F32, a.alpha = alpha, a.eps = eps;
+  a.r = d_r, a.ldr = ldr, a.h = d_h, a.ldh = ldh, a.rstd_z = d_rstd_z, a.rstd_r = d_rstd_r, a.mask = make_mask(p, d_rng);
+  a.n = n, a.d = d;
+  ProfScope prof("norm_residual_fwd", d, (hipStream_t)stream);
+  return norm_fwd<true>(a, dtype, (hipStream_t)stream);
+}
+
+int cg_norm_residual_bwd(const void *d_dr, int64_t lddr, const void *d_dh, int64_t lddh, const void *d_z, int64_t ldz,
+                         const void *d_r, int64_t ldr, const void *d_gate, int64_t ldgate, int gate_kind,
+                         const void *d_w_post, const void *d_w_pre, const void *d_scale, int wdtype, float alpha,
+                         double p, const int64_t *d_rng, const float *d_rstd_z, const float *d_rstd_r, void *d_dz,
+                         int64_t lddz, void *d_dx, int64_t lddx, void *d_dgate, int64_t lddgate, void *d_dw_post,
+                         void *d_dw_pre, void *d_dscale, int64_t n, int32_t d, int dtype, void *d_work,
+                         int64_t work_bytes, cg_stream_t stream) {
+  using namespace cg;
+  const char *who = "cg_norm_residual_bwd";
+  CG_TRY(check_dtype(who, dtype));
+  CG_TRY(check_weights(who, dtype, wdtype));
+  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_float(who, "alpha", alpha, false));
+  CG_TRY(check_p(who, p, d_rng));
+  if (gate_kind < CG_GATE_NONE || gate_kind > CG_GATE_FULL) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: gate kind %d", who, gate_kind);
+  if (n > 0) {
+    if ((!d_dr && !d_dh) || !d_z || !d_r || !d_rstd_z || !d_rstd_r || !d_dz || !d_dx || !d_work ||
+        (gate_kind != CG_GATE_NONE && (!d_gate || !d_dgate)))
+      CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
+    if ((d_dr && lddr < d) || (d_dh && lddh < d) || ldz < d || ldr < d || lddz < d || lddx < d ||
+        (gate_kind == CG_GATE_FULL && (ldgate < d || lddgate < d)) || (gate_kind == CG_GATE_ROW && (ldgate < 1 || lddgate < 1)))
+      CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
+    const void *ins[5] = {d_dr, d_dh, d_z, d_r, gate_kind != CG_GATE_NONE ? d_gate : nullptr};
+    const void *outs[3] = {d_dz, d_dx, gate_kind != CG_GATE_NONE ? d_dgate : nullptr};
+    for (int o = 0; o < 3; ++o) {
+      for (const void *i : ins)
+        if (outs[o] && outs[o] == i) CG_FAIL(CG_ERR_ALIAS, "%s: an output may not be an input", who);
+      if (outs[o] && outs[o] == outs[(o + 1) % 3]) CG_FAIL(CG_ERR_ALIAS, "%s: two outputs are the same", who);
+    }
+    if (work_bytes < (int64_t)norm_workspace(n, d)) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)norm_workspace(n, d));
+  }
+  NormArgs a = {};
+  a.dr = d_dr, a.lddr = lddr, a.dh = d_dh, a.lddh = lddh, a.z = d_z, a.ldz = ldz, a.r_in = d_r, a.ldr_in = ldr;
+  a.gate = d_gate, a.ldgate = ldgate, a.gate_kind = gate_kind, a.w_post = d_w_post, a.w_pre = d_w_pre, a.scale = d_scale;
+  a.w_f32 = wdtype == CG_F32, a.alpha = alpha, a.mask = make_mask(p, d_rng);
+  a.rstd_z = const_cast<float *>(d_rstd_z), a.rstd_r = const_cast<float *>(d_rstd_r);
+  a.dz = d_dz, a.lddz = lddz, a.dx = d_dx, a.lddx = lddx, a.dgate = d_dgate, a.lddgate = lddgate;
+  a.partial = (float *)d_work, a.n = n, a.d = d;
+  ProfScope prof("norm_residual_bwd", d, (hipStream_t)stream);
+  return norm_bwd<true>(a, dtype, d_dw_post, d_dw_pre, d_dscale, (hipStream_t)stream);
+}
+
+}  // extern "C"

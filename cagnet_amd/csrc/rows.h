@@ -1,0 +1,167 @@
+// Typed row access and the counter-based generator shared by the row-wise training operators (dropout, embedding,
+// rms_norm, norm_residual).  Activations are float32, bfloat16 or float16 in memory and float32 in registers.
+#pragma once
+#include "common.h"
+
+namespace cg {
+
+template <int DTYPE>
+struct Elem;
+template <>
+struct Elem<CG_F32> {
+  typedef float type;
+};
+template <>
+struct Elem<CG_BF16> {
+  typedef __bf16 type;
+};
+template <>
+struct Elem<CG_F16> {
+  typedef _Float16 type;
+};
+
+// N consecutive elements that are only aligned as single elements are: rows of 602 floats start 8 bytes apart from a
+// 16-byte boundary, rows of 41 start anywhere.  The memory pipeline takes wide accesses at any element address, so
+// such rows are moved 16 bytes per lane like aligned ones.
+template <typename T, int N>
+struct Pack {
+  typedef T type __attribute__((ext_vector_type(N), aligned(alignof(T))));
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_pack(const T *__restrict__ p, float (&out)[N]) {
+  const typename Pack<T, N>::type q = *reinterpret_cast<const typename Pack<T, N>::type *>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) out[i] = (float)q[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_pack(T *__restrict__ p, const float (&in)[N]) {
+  typename Pack<T, N>::type q;
+#pragma unroll
+  for (int i = 0; i < N; ++i) q[i] = (T)in[i];
+  *reinterpret_cast<typename Pack<T, N>::type *>(p) = q;
+}
+// the first `live` (0..N) of N elements; the others read as zero and are not written
+template <typename T, int N>
+__device__ __forceinline__ void load_some(const T *__restrict__ p, int live, float (&out)[N]) {
+  if (live >= N) {
+    load_pack<T, N>(p, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = i < live ? (float)p[i] : 0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_some(T *__restrict__ p, int live, const float (&in)[N]) {
+  if (live >= N) {
+    store_pack<T, N>(p, in);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < live) p[i] = (T)in[i];
+  }
+}
+
+// A weight vector: float32, or the type of the activations; a null pointer stands for ones.
+template <typename T>
+__device__ __forceinline__ float weight_at(const void *w, int w_f32, int32_t j) {
+  if (!w) return 1.f;
+  return w_f32 ? static_cast<const float *>(w)[j] : (float)static_cast<const T *>(w)[j];
+}
+template <typename T>
+__device__ __forceinline__ void weight_put(void *w, int w_f32, int32_t j, float v) {
+  if (w_f32)
+    static_cast<float *>(w)[j] = v;
+  else
+    static_cast<T *>(w)[j] = (T)v;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Masks.  Philox 4x32 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3",
+// 2011): a keyed bijection of a 128-bit counter, each round two 32 x 32 -> 64 bit products.  Seven
+// rounds are the fewest for which the paper reports no failure in its statistical test batteries;
+// its default of ten adds a margin that a mask of kept elements has no use for, and costs as much
+// again per element as the rest of the kernel at 2 bytes an element.
+//   key = the seed; counter = (column / 4, row, offset low, offset high); word column % 4 of the
+// result decides element (row, column), whatever the strides, the type or the kernel that asks.
+// ---------------------------------------------------------------------------------------------
+constexpr int kPhiloxRounds = 7;
+
+struct Mask {  // what the host knows of a dropout: `last` is the largest word that still drops
+  const int64_t *rng;  // device {seed, offset}; nullptr: nothing is dropped
+  uint32_t last;
+  float inv_keep;  // 1 / (1 - p)
+};
+
+// p = 0: nothing to drop (no mask at all).  p = 1: every word drops.
+static inline Mask make_mask(double p, const int64_t *d_rng) {
+  const double t = p * 4294967296.0 + 0.5;
+  const uint64_t threshold = t >= 4294967296.0 ? (1ull << 32) : (uint64_t)t;
+  Mask m;
+  m.rng = threshold > 0 ? d_rng : nullptr;
+  m.last = threshold > 0 ? (uint32_t)(threshold - 1) : 0u;
+  m.inv_keep = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
+  return m;
+}
+
+struct MaskKey {
+  uint32_t seed_lo, seed_hi, off_lo, off_hi;
+};
+__device__ __forceinline__ MaskKey mask_key(const int64_t *__restrict__ rng) {
+  const uint64_t seed = (uint64_t)rng[0], off = (uint64_t)rng[1];
+  return MaskKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
+}
+
+// the four words of columns 4 * block .. 4 * block + 3 of `row`
+__device__ __forceinline__ void mask_words(const MaskKey &k, uint32_t row, uint32_t block, uint32_t (&w)[4]) {
+  uint32_t c0 = block, c1 = row, c2 = k.off_lo, c3 = k.off_hi, k0 = k.seed_lo, k1 = k.seed_hi;
+#pragma unroll
+  for (int r = 0; r < kPhiloxRounds; ++r) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c1 = (uint32_t)b;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  w[0] = c0;
+  w[1] = c1;
+  w[2] = c2;
+  w[3] = c3;
+}
+// 1 / (1 - p) for a kept element, 0 for a dropped one; one element at a time
+__device__ __forceinline__ float mask_at(const MaskKey &k, const Mask &m, int64_t row, int32_t j) {
+  uint32_t w[4];
+  mask_words(k, (uint32_t)row, (uint32_t)j >> 2, w);
+  const uint32_t mine = (j & 2) ? ((j & 1) ? w[3] : w[2]) : ((j & 1) ? w[1] : w[0]);
+  return mine > m.last ? m.inv_keep : 0.f;
+}
+
+// ---- argument checks shared by the entry points ---------------------------------------------------
+static inline int check_dtype(const char *who, int dtype) {
+  if (dtype != CG_F32 && dtype != CG_BF16 && dtype != CG_F16)
+    CG_FAIL(CG_ERR_UNSUPPORTED, "%s: dtype %d is none of CG_F32, CG_BF16, CG_F16", who, dtype);
+  return CG_OK;
+}
+static inline int check_row_shape(const char *who, int64_t n, int32_t d) {
+  if (n < 0 || d <= 0) CG_FAIL(CG_ERR_SIZE, "%s: n=%lld rows of d=%d elements", who, (long long)n, d);
+  if (n > 0xffffffffLL) CG_FAIL(CG_ERR_OVERFLOW, "%s: n=%lld rows (at most 2^32 - 1)", who, (long long)n);
+  return CG_OK;
+}
+static inline int check_p(const char *who, double p, const int64_t *d_rng) {
+  if (!(p >= 0.0 && p <= 1.0)) CG_FAIL(CG_ERR_SIZE, "%s: dropout probability %g outside [0, 1]", who, p);
+  if (p > 0.0 && !d_rng) CG_FAIL(CG_ERR_NULL, "%s: p > 0 without generator state", who);
+  return CG_OK;
+}
+static inline size_t elem_size(int dtype) { return dtype == CG_F32 ? 4 : 2; }
+
+// calls F<dtype constant>
+#define CG_BY_DTYPE(dtype, CALL)          \
+  switch (dtype) {                        \
+    case CG_F32: CALL(CG_F32); break;     \
+    case CG_BF16: CALL(CG_BF16); break;   \
+    default: CALL(CG_F16); break;         \
+  }
+
+}  // namespace cg

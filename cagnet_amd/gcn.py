@@ -19,6 +19,7 @@ from typing import List, Optional, Sequence, Union
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .ops import CsrMatrix
@@ -384,11 +385,126 @@ class LogSoftmaxNLLLoss(torch.autograd.Function):
         return dz, None, None
 
 
-def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank=0, size=1, group=None):
+# ------------------------------------------------------------------------------------------------
+# Row-wise training operators as autograd nodes: what a stack of GCNFunc layers needs around them when it gets
+# deeper than the reference's two layers (which have no counterpart of these):
+#   x = dropout(embedding(table, ids), p, rng_next(state));  h = rms_norm(x, w_0)
+#   z = GCNFunc.apply(h, W_k, ...);  x, h = norm_residual(z, x, w_post, w_pre, gate, scale)      for every layer k
+# First derivatives only.
+# ------------------------------------------------------------------------------------------------
+rng_state, rng_next = ops.rng_state, ops.rng_next
+
+
+class Dropout(torch.autograd.Function):
+    """ops.dropout_fwd / dropout_bwd; only the generator's snapshot is kept between them."""
+
+    @staticmethod
+    def forward(ctx, x, p, rng):
+        ctx.p, ctx.has_rng = p, rng is not None
+        ctx.save_for_backward(*([rng] if rng is not None else []))
+        return ops.dropout_fwd(x, p, rng)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return ops.dropout_bwd(g, ctx.p, ctx.saved_tensors[0] if ctx.has_rng else None), None, None
+
+
+def dropout(x: torch.Tensor, p: float, rng: Optional[torch.Tensor]) -> torch.Tensor:
+    """x / (1 - p) where kept, 0 elsewhere; `rng` is a snapshot from `rng_next`, one for every dropout of a step.
+    A `rng` that is stepped or written before the gradient ran is refused by autograd's version check."""
+    return Dropout.apply(x, p, rng)
+
+
+class Embedding(torch.autograd.Function):
+    """ops.embedding_fwd / embedding_bwd."""
+
+    @staticmethod
+    def forward(ctx, table, idx, scale):
+        flat = idx.reshape(-1)
+        ctx.save_for_backward(flat)
+        ctx.rows, ctx.width, ctx.scale = table.shape[0], table.shape[1], scale
+        return ops.embedding_fwd(table, flat, scale).view(*idx.shape, table.shape[1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        (flat,) = ctx.saved_tensors
+        return ops.embedding_bwd(g.reshape(-1, ctx.width), flat, ctx.rows, ctx.scale), None, None
+
+
+def embedding(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[idx] for indices of any shape; an index outside the table reads zeros and gets no gradient."""
+    return Embedding.apply(table, idx, float(scale))
+
+
+class RmsNorm(torch.autograd.Function):
+    """ops.rms_norm_fwd / rms_norm_bwd."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        y, rstd = ops.rms_norm_fwd(x, weight, eps)
+        ctx.save_for_backward(x, rstd, *([weight] if weight is not None else []))
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, rstd, *weight = ctx.saved_tensors
+        dx, dw = ops.rms_norm_bwd(g, x, weight[0] if weight else None, rstd)
+        return dx, dw, None
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6) -> torch.Tensor:
+    """x / sqrt(mean of x^2 over the row + eps) * weight."""
+    return RmsNorm.apply(x, weight, eps)
+
+
+class NormResidual(torch.autograd.Function):
+    """ops.norm_residual_fwd / norm_residual_bwd."""
+
+    @staticmethod
+    def forward(ctx, z, x, w_post, w_pre, gate, scale, alpha, p, rng, eps):
+        r, h, rstd_z, rstd_r = ops.norm_residual_fwd(z, x, w_post, w_pre, gate, scale, alpha, p, rng, eps)
+        maybe = (w_post, w_pre, gate, scale, rng)
+        ctx.have = [t is not None for t in maybe]
+        ctx.save_for_backward(z, r, rstd_z, rstd_r, *[t for t in maybe if t is not None])
+        ctx.alpha, ctx.p = alpha, p
+        ctx.set_materialize_grads(False)
+        return r, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dh):
+        if dr is None and dh is None:
+            return (None,) * 10
+        z, r, rstd_z, rstd_r, *rest = ctx.saved_tensors
+        rest = iter(rest)
+        w_post, w_pre, gate, scale, rng = (next(rest) if have else None for have in ctx.have)
+        dz, dx, dgate, dw_post, dw_pre, dscale = ops.norm_residual_bwd(dr, dh, z, r, w_post, w_pre, rstd_z, rstd_r, gate,
+                                                                       scale, ctx.alpha, ctx.p, rng)
+        return dz, dx, dw_post, dw_pre, dgate, dscale, None, None, None, None
+
+
+def norm_residual(z: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tensor], w_pre: Optional[torch.Tensor],
+                  gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                  p: float = 0.0, rng: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """(r, h): r = x + alpha * scale * dropout(sigmoid(gate) * rms_norm(z, w_post)), h = rms_norm(r, w_pre)."""
+    return NormResidual.apply(z, x, w_post, w_pre, gate, scale, alpha, p, rng, eps)
+
+
+def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank=0, size=1, group=None,
+          dropout_p: float = 0.0, rng: Optional[torch.Tensor] = None):
     """One epoch, gcn_distr.py:341-366.  `data` needs `.y` and `.train_mask`; `group` is None for a
-    whole graph on one GPU, or a pair (layer-1 ResidentBlocks, layer-2 ResidentBlocks)."""
+    whole graph on one GPU, or a pair (layer-1 ResidentBlocks, layer-2 ResidentBlocks).  dropout_p > 0 drops
+    hidden activations between the two layers (the reference has none); `rng` is then the generator state
+    (`rng_state`), which every epoch steps once."""
     g1, g2 = group if isinstance(group, (tuple, list)) else (group, group)
+    if dropout_p > 0.0 and rng is None:
+        raise ValueError("train: dropout_p > 0 needs a generator state (rng)")
     outputs = GCNFunc.apply(inputs, weight1, adj_matrix, am_partitions, rank, size, g1, F.relu)
+    if dropout_p > 0.0:
+        outputs = dropout(outputs, dropout_p, rng_next(rng))
     fuse = fused_loss and activations
     outputs = GCNFunc.apply(outputs, weight2, adj_matrix, am_partitions, rank, size, g2, None if fuse else F.log_softmax)
 
@@ -425,6 +541,7 @@ class GraphedTrain:
     replays it.  Every tensor the epoch reads (`inputs`, the weights, `data.y`, `data.train_mask`)
     is read from the same memory on every replay: update them in place.  Optimizers that keep
     scalars on the host must be built for capture (`torch.optim.Adam(..., capturable=True)`).
+    With `dropout_p` the generator state `rng` is read and stepped on the device: every replay draws a new mask.
 
     The graph replays with the addresses of the library's scratch buffers of its stream and of the
     tables of the matrices it multiplies with; the library keeps both alive for as long as the matrices
@@ -434,10 +551,10 @@ class GraphedTrain:
     `graph_release`)."""
 
     def __init__(self, inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank=0, size=1,
-                 group=None, warmup: int = 3):
+                 group=None, warmup: int = 3, dropout_p: float = 0.0, rng: Optional[torch.Tensor] = None):
         if warmup < 1:
             raise ValueError("at least one warm-up epoch is needed: it builds the schedules and grows the scratch")
-        args = (inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank, size, group)
+        args = (inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank, size, group, dropout_p, rng)
         self.stream = torch.cuda.Stream(device=weight1.device)
         self.stream.wait_stream(torch.cuda.current_stream(weight1.device))
         with torch.cuda.stream(self.stream):

@@ -2,7 +2,8 @@
 every computation happens in libcagnet_amd.so.
 
 Dense operands are fp32 CUDA(HIP) tensors, row-major with unit column stride (a row stride larger
-than the column count is passed on as the leading dimension).  Sparse indices are int32.
+than the column count is passed on as the leading dimension).  Sparse indices are int32.  The row-wise
+training operators (dropout, embedding, rms_norm, norm_residual) also take bfloat16 and float16.
 """
 from __future__ import annotations
 
@@ -19,6 +20,8 @@ __all__ = [
     "CagnetError", "CsrMatrix", "coo2csr_rowptr", "coo2csr", "csr_transpose", "coo_check", "spmm_coo",
     "dense_xw", "dense_gwt", "dense_xtg", "relu_fwd", "relu_bwd", "log_softmax_fwd", "log_softmax_bwd",
     "nll_loss_fwd", "nll_loss_bwd", "log_softmax_nll_bwd",
+    "rng_state", "rng_next", "dropout_fwd", "dropout_bwd", "embedding_fwd", "embedding_bwd", "rms_norm_fwd",
+    "rms_norm_bwd", "norm_residual_fwd", "norm_residual_bwd",
 ]
 
 
@@ -623,6 +626,321 @@ def log_softmax_nll_bwd(logp: torch.Tensor, y: torch.Tensor, mask: Optional[torc
                                      c_void_p(gs.data_ptr()) if gs is not None else c_void_p(0), _ptr(dz), max(c, 1),
                                      n, c, _stream()), "cg_log_softmax_nll_bwd")
     return dz
+
+
+# ------------------------------------------------------------------------------------------------
+# row-wise training operators: dropout, embedding lookup, norms, the residual block around a layer.
+# Activations are float32, bfloat16 or float16; weights are float32 or have the activations' type.
+# Temporary memory comes from torch's allocator, so that a captured graph owns its own.
+# ------------------------------------------------------------------------------------------------
+_ROW_DTYPES = {torch.float32: _lib.CG_F32, torch.bfloat16: _lib.CG_BF16, torch.float16: _lib.CG_F16}
+
+
+class _On:
+    """The device and stream a call runs on: those of its operands, whatever device is current."""
+
+    __slots__ = ("device", "guard", "stream")
+
+    def __init__(self, t: torch.Tensor):
+        self.device = t.device
+        self.guard = None
+
+    def __enter__(self):
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        self.stream = torch.cuda.current_stream(self.device).cuda_stream
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, int]:
+    """(tensor, leading dimension) of an [n, d] activation; with `like`, of its shape, type and device.
+    Copies only when the column stride is not 1 or rows overlap."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must live on the GPU (got device {t.device}); there is no CPU path")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name}: expected dtype {like.dtype}, got {t.dtype}")
+        if t.shape != like.shape:
+            raise ValueError(f"{name}: expected shape {tuple(like.shape)}, got {tuple(t.shape)}")
+        if t.device != like.device:
+            raise ValueError(f"{name}: on {t.device}, the other operands are on {like.device}")
+    elif t.dtype not in _ROW_DTYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    elif t.dim() != 2:
+        raise ValueError(f"{name}: expected 2 dimensions, got {t.dim()}")
+    rows, cols = t.shape
+    if cols == 0:
+        raise ValueError(f"{name}: rows of no elements")
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t, max(t.stride(0) if rows > 1 else cols, cols)
+
+
+def _weights(x: torch.Tensor, **named: Optional[torch.Tensor]):
+    """The given [d] weights (None = ones), contiguous, and their common dtype."""
+    dtype = None
+    out = []
+    for name, w in named.items():
+        if w is not None:
+            if not isinstance(w, torch.Tensor):
+                raise TypeError(f"{name}: expected a torch.Tensor, got {type(w).__name__}")
+            if w.dtype != torch.float32 and w.dtype != x.dtype:
+                raise TypeError(f"{name}: expected dtype float32 or {x.dtype}, got {w.dtype}")
+            if dtype is not None and w.dtype != dtype:
+                raise TypeError(f"{name}: weights of one call share a dtype, got {w.dtype} beside {dtype}")
+            if w.dim() != 1 or w.shape[0] != x.shape[1]:
+                raise ValueError(f"{name}: expected shape ({x.shape[1]},), got {tuple(w.shape)}")
+            if w.device != x.device:
+                raise ValueError(f"{name}: on {w.device}, the other operands are on {x.device}")
+            dtype = w.dtype
+            w = w if w.is_contiguous() else w.contiguous()
+        out.append(w)
+    return (*out, torch.float32 if dtype is None else dtype)
+
+
+def _row_stats(t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
+    t = _need(t, name, torch.float32, 1)
+    if t.shape[0] != x.shape[0] or t.device != x.device:
+        raise ValueError(f"{name}: expected {x.shape[0]} entries on {x.device}, got {t.shape[0]} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _probability(p: float, rng: Optional[torch.Tensor], x: torch.Tensor) -> float:
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p: dropout probability {p} outside [0, 1]")
+    if p > 0.0:
+        if rng is None:
+            raise ValueError("rng: p > 0 needs a generator state (ops.rng_state, ops.rng_next)")
+        _need_rng(rng, "rng", x.device)
+    return p
+
+
+def _need_rng(rng: torch.Tensor, name: str, device=None) -> torch.Tensor:
+    rng = _need(rng, name, torch.int64, 1)
+    if rng.numel() != 2 or not rng.is_contiguous():
+        raise ValueError(f"{name}: a generator state is a contiguous int64 tensor of 2, got {tuple(rng.shape)}")
+    if device is not None and rng.device != device:
+        raise ValueError(f"{name}: on {rng.device}, the other operands are on {device}")
+    return rng
+
+
+def _workspace(query, where: str, device, *sizes) -> torch.Tensor:
+    need = ctypes.c_int64(0)
+    check(query(*sizes, ctypes.byref(need)), where)
+    return torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+
+
+def rng_state(seed: int, device="cuda:0", offset: int = 0) -> torch.Tensor:
+    """State of the dropout generator, int64 {seed, offset} on the device.  It lives in device memory so that a
+    captured graph draws new masks on every replay: `rng_next` inside the graph steps it."""
+    wrap = lambda v: ((int(v) + (1 << 63)) % (1 << 64)) - (1 << 63)  # noqa: E731  (64 bits, whatever the sign)
+    return torch.tensor([wrap(seed), wrap(offset)], dtype=torch.int64, device=device)
+
+
+def rng_next(state: torch.Tensor) -> torch.Tensor:
+    """A snapshot of `state` for one dropout (its forward pass and its gradient), and `state` steps on."""
+    state = _need_rng(state, "state")
+    snapshot = torch.empty_like(state)
+    with _On(state) as on:
+        torch.autograd.graph.increment_version(state)
+        check(lib.cg_rng_next(state.data_ptr(), snapshot.data_ptr(), on.stream), "cg_rng_next")
+    return snapshot
+
+
+def _dropout(x: torch.Tensor, p: float, rng: Optional[torch.Tensor], name: str) -> torch.Tensor:
+    x, ldx = _rows(x, name)
+    p = _probability(p, rng, x)
+    n, d = x.shape
+    out = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    with _On(x) as on:
+        check(lib.cg_dropout(x.data_ptr(), ldx, out.data_ptr(), d, n, d, _ROW_DTYPES[x.dtype], p, _at(rng), on.stream),
+              "cg_dropout")
+    return out
+
+
+def dropout_fwd(x: torch.Tensor, p: float, rng: Optional[torch.Tensor]) -> torch.Tensor:
+    """x / (1 - p) where the element is kept, 0 elsewhere.  The mask is a function of rng = {seed, offset}, row and
+    column (Philox 4x32-7; cg_dropout in the header gives the definition) and is never stored."""
+    return _dropout(x, p, rng, "x")
+
+
+def dropout_bwd(g: torch.Tensor, p: float, rng: Optional[torch.Tensor]) -> torch.Tensor:
+    """Gradient of dropout_fwd with the same p and rng: the mask is computed again."""
+    return _dropout(g, p, rng, "g")
+
+
+def _lookup_indices(idx: torch.Tensor, device) -> torch.Tensor:
+    if not isinstance(idx, torch.Tensor):
+        raise TypeError(f"idx: expected a torch.Tensor, got {type(idx).__name__}")
+    if idx.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"idx: expected dtype int32 or int64, got {idx.dtype}")
+    if idx.dim() != 1:
+        raise ValueError(f"idx: expected 1 dimension, got {idx.dim()}")
+    if idx.device != device:
+        raise ValueError(f"idx: on {idx.device}, the other operands are on {device}")
+    return idx if idx.is_contiguous() else idx.contiguous()
+
+
+def embedding_fwd(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[idx]; an index outside the table gives a row of zeros (padding)."""
+    table, ldt = _rows(table, "table")
+    idx = _lookup_indices(idx, table.device)
+    rows, d = table.shape
+    n = idx.shape[0]
+    out = torch.empty((n, d), dtype=table.dtype, device=table.device)
+    with _On(table) as on:
+        check(lib.cg_embedding_fwd(table.data_ptr(), ldt, rows, idx.data_ptr(), int(idx.dtype == torch.int64), n, d,
+                                   _ROW_DTYPES[table.dtype], float(scale), out.data_ptr(), d, on.stream),
+              "cg_embedding_fwd")
+    return out
+
+
+def embedding_bwd(g: torch.Tensor, idx: torch.Tensor, rows: int, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+                  beta: float = 0.0) -> torch.Tensor:
+    """Gradient of the table of embedding_fwd: out_v = scale * sum of g_i over idx_i == v, + beta * out_v.  A fresh
+    output of g's type is allocated (and beta forced to 0) if none is given; a given one may also be float32.
+    Same bits on every call: the positions are sorted by index and added up in a fixed order."""
+    g, ldg = _rows(g, "g")
+    idx = _lookup_indices(idx, g.device)
+    n, d = g.shape
+    if idx.shape[0] != n:
+        raise ValueError(f"idx has {idx.shape[0]} entries for {n} rows of g")
+    rows = int(rows)
+    if out is None:
+        out = torch.empty((max(rows, 0), d), dtype=g.dtype, device=g.device)
+        beta = 0.0
+    else:
+        if not isinstance(out, torch.Tensor):
+            raise TypeError(f"out: expected a torch.Tensor, got {type(out).__name__}")
+        if out.dtype != g.dtype and out.dtype != torch.float32:
+            raise TypeError(f"out: expected dtype {g.dtype} or float32, got {out.dtype}")
+        if tuple(out.shape) != (rows, d) or out.device != g.device:
+            raise ValueError(f"out: expected shape {(rows, d)} on {g.device}, got {tuple(out.shape)} on {out.device}")
+        if (d > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < d):
+            raise ValueError(f"out: output must be row-major with unit column stride (strides {out.stride()})")
+        torch.autograd.graph.increment_version(out)
+    ldo = max(out.stride(0) if rows > 1 else d, d)
+    work = _workspace(lib.cg_embedding_bwd_workspace, "cg_embedding_bwd_workspace", g.device, n, rows, d)
+    with _On(g) as on:
+        check(lib.cg_embedding_bwd(g.data_ptr(), ldg, idx.data_ptr(), int(idx.dtype == torch.int64), n, rows, d,
+                                   _ROW_DTYPES[g.dtype], _ROW_DTYPES[out.dtype], float(scale), float(beta),
+                                   out.data_ptr(), ldo, work.data_ptr(), work.numel(), on.stream), "cg_embedding_bwd")
+    return out
+
+
+def rms_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, rstd): y = x * rstd * weight with rstd = 1 / sqrt(mean of x^2 over the row + eps), float32 [n]."""
+    x, ldx = _rows(x, "x")
+    w, wdtype = _weights(x, weight=weight)
+    n, d = x.shape
+    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    rstd = torch.empty(n, dtype=torch.float32, device=x.device)
+    with _On(x) as on:
+        check(lib.cg_rms_norm_fwd(x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], y.data_ptr(), d, rstd.data_ptr(), n, d,
+                                  _ROW_DTYPES[x.dtype], float(eps), on.stream), "cg_rms_norm_fwd")
+    return y, rstd
+
+
+def rms_norm_bwd(g: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], rstd: torch.Tensor):
+    """(dx, dweight) of rms_norm_fwd for the gradient g of y; dweight is None without a weight."""
+    x, ldx = _rows(x, "x")
+    g, ldg = _rows(g, "g", x)
+    w, wdtype = _weights(x, weight=weight)
+    rstd = _row_stats(rstd, "rstd", x)
+    n, d = x.shape
+    dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    dw = torch.empty_like(w) if w is not None else None
+    work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", x.device, n, d)
+    with _On(x) as on:
+        check(lib.cg_rms_norm_bwd(g.data_ptr(), ldg, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], rstd.data_ptr(),
+                                  dx.data_ptr(), d, _at(dw), n, d, _ROW_DTYPES[x.dtype], work.data_ptr(), work.numel(),
+                                  on.stream), "cg_rms_norm_bwd")
+    return dx, dw
+
+
+def _gate(gate: Optional[torch.Tensor], x: torch.Tensor):
+    """(tensor, leading dimension, kind) of a gate: None, one value per row [n, 1], or one per element [n, d]."""
+    if gate is None:
+        return None, 0, _lib.CG_GATE_NONE
+    if isinstance(gate, torch.Tensor) and gate.dim() == 2 and tuple(gate.shape) == (x.shape[0], 1):
+        gate, ld = _rows(gate, "gate", gate if gate.dtype == x.dtype and gate.device == x.device else x)
+        return gate, ld, _lib.CG_GATE_ROW
+    gate, ld = _rows(gate, "gate", x)
+    return gate, ld, _lib.CG_GATE_FULL
+
+
+def norm_residual_fwd(z: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tensor], w_pre: Optional[torch.Tensor],
+                      gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, alpha: float = 1.0,
+                      p: float = 0.0, rng: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """(r, h, rstd_z, rstd_r): the residual sum behind a block with input stream x and output z, and the norm in
+    front of the next block, in one pass:
+        r = x + alpha * scale * dropout(sigmoid(gate) * rms_norm(z, w_post)),   h = rms_norm(r, w_pre)
+    w_post, w_pre, scale: [d] or None (ones); gate: None, [n, 1] or [n, d], before the sigmoid; p, rng as in
+    dropout_fwd (the same mask).  h is taken from the sum before it is rounded to z's type."""
+    z, ldz = _rows(z, "z")
+    x, ldx = _rows(x, "x", z)
+    gate, ldg, kind = _gate(gate, z)
+    w_post, w_pre, scale, wdtype = _weights(z, w_post=w_post, w_pre=w_pre, scale=scale)
+    p = _probability(p, rng, z)
+    n, d = z.shape
+    r = torch.empty((n, d), dtype=z.dtype, device=z.device)
+    h = torch.empty_like(r)
+    rstd_z = torch.empty(n, dtype=torch.float32, device=z.device)
+    rstd_r = torch.empty_like(rstd_z)
+    with _On(z) as on:
+        check(lib.cg_norm_residual_fwd(z.data_ptr(), ldz, x.data_ptr(), ldx, _at(gate), ldg, kind, _at(w_post), _at(w_pre),
+                                       _at(scale), _ROW_DTYPES[wdtype], float(alpha), p, _at(rng), float(eps),
+                                       r.data_ptr(), d, h.data_ptr(), d, rstd_z.data_ptr(), rstd_r.data_ptr(), n, d,
+                                       _ROW_DTYPES[z.dtype], on.stream), "cg_norm_residual_fwd")
+    return r, h, rstd_z, rstd_r
+
+
+def norm_residual_bwd(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], z: torch.Tensor, r: torch.Tensor,
+                      w_post: Optional[torch.Tensor], w_pre: Optional[torch.Tensor], rstd_z: torch.Tensor,
+                      rstd_r: torch.Tensor, gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
+                      alpha: float = 1.0, p: float = 0.0, rng: Optional[torch.Tensor] = None):
+    """(dz, dx, dgate, dw_post, dw_pre, dscale) of norm_residual_fwd for the gradients dr of r and dh of h (either may
+    be None: zero); entries whose input was None are None."""
+    z, ldz = _rows(z, "z")
+    if dr is None and dh is None:
+        raise ValueError("dr, dh: at least one gradient has to be given")
+    lddr = lddh = 0
+    if dr is not None:
+        dr, lddr = _rows(dr, "dr", z)
+    if dh is not None:
+        dh, lddh = _rows(dh, "dh", z)
+    r, ldr = _rows(r, "r", z)
+    gate, ldg, kind = _gate(gate, z)
+    w_post, w_pre, scale, wdtype = _weights(z, w_post=w_post, w_pre=w_pre, scale=scale)
+    rstd_z, rstd_r = _row_stats(rstd_z, "rstd_z", z), _row_stats(rstd_r, "rstd_r", z)
+    p = _probability(p, rng, z)
+    n, d = z.shape
+    dz = torch.empty((n, d), dtype=z.dtype, device=z.device)
+    dx = torch.empty_like(dz)
+    dgate = torch.empty(gate.shape, dtype=z.dtype, device=z.device) if gate is not None else None
+    dw_post, dw_pre, dscale = (torch.empty_like(w) if w is not None else None for w in (w_post, w_pre, scale))
+    work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", z.device, n, d)
+    with _On(z) as on:
+        check(lib.cg_norm_residual_bwd(_at(dr), lddr, _at(dh), lddh, z.data_ptr(), ldz, r.data_ptr(), ldr, _at(gate), ldg,
+                                       kind, _at(w_post), _at(w_pre), _at(scale), _ROW_DTYPES[wdtype], float(alpha), p,
+                                       _at(rng), rstd_z.data_ptr(), rstd_r.data_ptr(), dz.data_ptr(), d, dx.data_ptr(), d,
+                                       _at(dgate), dgate.shape[1] if dgate is not None else 0, _at(dw_post), _at(dw_pre),
+                                       _at(dscale), n, d, _ROW_DTYPES[z.dtype], work.data_ptr(), work.numel(), on.stream),
+              "cg_norm_residual_bwd")
+    return dz, dx, dgate, dw_post, dw_pre, dscale
 
 
 # A wide dense operand whose rows are not a whole number of 128-byte lines long (602 floats = 2408 bytes) is read by the

@@ -281,6 +281,81 @@ int cg_log_softmax_nll_fwd(const float *d_z, int64_t ldz, const int64_t *d_y, co
                            int64_t ldo, int64_t n, int32_t c, float *d_loss, int64_t *d_count, cg_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Row-wise training operators on activations of float32, bfloat16 or float16 (`dtype`): dropout,
+ * embedding lookup, norms and the residual block around a layer.  The reference trains without
+ * them (no counterpart; its layers end in F.relu / F.log_softmax, gcn_distr.py:284-294).
+ * Arithmetic is float32 whatever the type, rounded once at each store.  Weight vectors ([d], NULL =
+ * ones) and their gradients are float32 or have the activations' type (`wdtype`, one for all).
+ * n rows (at most 2^32 - 1) of d columns; n == 0 is legal (weight gradients are then zero).
+ * Outputs may not overlap inputs (cg_dropout may run in place).  Nothing is allocated and nothing is
+ * read back: the gradients that need temporary memory take it from the caller (`d_work`, at least the
+ * size the matching *_workspace function names, 16-byte aligned), so that every call can be captured
+ * into a HIP graph, the first one included, and graphs captured with workspaces of their own may
+ * replay side by side.
+ */
+enum cg_dtype { CG_F32 = 0, CG_BF16 = 1, CG_F16 = 2 };
+enum cg_gate_kind { CG_GATE_NONE = 0, CG_GATE_ROW = 1, CG_GATE_FULL = 2 };
+
+/* Snapshot of a dropout generator's state and step to the next one: out = state = {seed, offset},
+ * then state.offset += 1.  A forward pass and its gradient take the same snapshot; no counterpart in
+ * the reference. */
+int cg_rng_next(int64_t *d_state, int64_t *d_out, cg_stream_t stream);
+
+/* out = keep ? x / (1 - p) : 0, and the gradient of the same (x is then the incoming gradient).
+ * 0 <= p <= 1.  The mask is a function of {seed, offset} (d_rng, device), row and column alone: word
+ * column % 4 of Philox 4x32-7 with key = seed and counter = (column / 4, row, offset low, offset high)
+ * drops its element when it is below floor(p 2^32 + 1/2).  It depends on neither strides nor type, so
+ * the gradient recomputes it and nothing is stored.  d_rng may be NULL when p == 0 (out = x).  d_out
+ * may be d_x when the leading dimensions are equal.  No counterpart in the reference. */
+int cg_dropout(const void *d_x, int64_t ldx, void *d_out, int64_t ldo, int64_t n, int32_t d, int dtype, double p,
+               const int64_t *d_rng, cg_stream_t stream);
+
+/* out_i = scale * table[idx_i] for n indices (int32, or int64 when idx64 != 0) into `rows` rows; an
+ * index outside [0, rows) gives a row of zeros (padding).  No counterpart in the reference. */
+int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void *d_idx, int idx64, int64_t n, int32_t d,
+                     int dtype, float scale, void *d_out, int64_t ldo, cg_stream_t stream);
+/* Its gradient, out_v = scale * sum_{i: idx_i = v} g_i + beta * out_v for every table row v (rows no index
+ * names get beta * out_v, and are neither read nor written when beta == 1; beta == 0 never reads out).
+ * out has the type of g or is float32 (`out_dtype`).  Indices outside the table add to nothing.  The
+ * additions of a row run in a fixed order that depends on the indices alone. */
+int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *bytes);
+int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64, int64_t n, int64_t rows, int32_t d,
+                     int dtype, int out_dtype, float scale, float beta, void *d_out, int64_t ldo, void *d_work,
+                     int64_t work_bytes, cg_stream_t stream);
+
+/* y = x rstd w with rstd = 1 / sqrt(mean over the row of x^2 + eps), eps > 0; rstd is written for the
+ * gradient dx = rstd (g w - x rstd mean(g w x rstd)), dw = sum over rows of g x rstd (d_dw nullable).
+ * No counterpart in the reference. */
+int cg_rms_norm_fwd(const void *d_x, int64_t ldx, const void *d_w, int wdtype, void *d_y, int64_t ldy, float *d_rstd,
+                    int64_t n, int32_t d, int dtype, float eps, cg_stream_t stream);
+int cg_norm_bwd_workspace(int64_t n, int32_t d, int64_t *bytes); /* of both gradients below */
+int cg_rms_norm_bwd(const void *d_g, int64_t ldg, const void *d_x, int64_t ldx, const void *d_w, int wdtype,
+                    const float *d_rstd, void *d_dx, int64_t lddx, void *d_dw, int64_t n, int32_t d, int dtype,
+                    void *d_work, int64_t work_bytes, cg_stream_t stream);
+
+/* The residual sum behind a block with output z, and the norm in front of the next block, in one pass:
+ *   r = x + alpha scale * drop(sigmoid(gate) * rms_norm(z, w_post)),   h = rms_norm(r, w_pre)
+ * gate: none, one value per row (CG_GATE_ROW, d_gate[row * ldgate]) or one per element (CG_GATE_FULL).
+ * drop: cg_dropout with probability p and generator state d_rng (p == 0: nothing dropped).  h is taken
+ * from the sum before its rounding to `dtype`.  rstd_z, rstd_r (n floats each) are kept for the gradient.
+ * No counterpart in the reference. */
+int cg_norm_residual_fwd(const void *d_z, int64_t ldz, const void *d_x, int64_t ldx, const void *d_gate, int64_t ldgate,
+                         int gate_kind, const void *d_w_post, const void *d_w_pre, const void *d_scale, int wdtype,
+                         float alpha, double p, const int64_t *d_rng, float eps, void *d_r, int64_t ldr, void *d_h,
+                         int64_t ldh, float *d_rstd_z, float *d_rstd_r, int64_t n, int32_t d, int dtype,
+                         cg_stream_t stream);
+/* Gradients of all of its inputs from those of r and h (either may be NULL = zero, not both): dz, dx, dgate
+ * (shaped as the gate; required with one), dw_post, dw_pre, dscale (each nullable).  r, rstd_z and rstd_r
+ * are the forward pass's. */
+int cg_norm_residual_bwd(const void *d_dr, int64_t lddr, const void *d_dh, int64_t lddh, const void *d_z, int64_t ldz,
+                         const void *d_r, int64_t ldr, const void *d_gate, int64_t ldgate, int gate_kind,
+                         const void *d_w_post, const void *d_w_pre, const void *d_scale, int wdtype, float alpha,
+                         double p, const int64_t *d_rng, const float *d_rstd_z, const float *d_rstd_r, void *d_dz,
+                         int64_t lddz, void *d_dx, int64_t lddx, void *d_dgate, int64_t lddgate, void *d_dw_post,
+                         void *d_dw_pre, void *d_dscale, int64_t n, int32_t d, int dtype, void *d_work,
+                         int64_t work_bytes, cg_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * A sparse block as one byte string in host memory, for files and for transfers between ranks.
  * The reference loads its adjacency matrix from a pickled int64 COO tensor (gcn_distr.py:747)
  * and sends blocks as three float32 arrays, indices included (gcn_distr_2d.py:369-374), which is
@@ -342,7 +417,8 @@ int cg_coo_block(const int32_t *d_row, const int32_t *d_col, const float *d_val,
  * partial rows), "spmm_panel_dense" (its dense tiles on the matrix cores), "spmm_panel_add" (partial rows added to a narrow
  * product), "dense_xw", "dense_gwt", "dense_xtg" (partial products and their sum),
  * "relu_fwd", "relu_bwd" (no suffix), "log_softmax_fwd", "log_softmax_bwd", "nll_fwd", "nll_bwd",
- * "log_softmax_nll_bwd".
+ * "log_softmax_nll_bwd", and with the row length d: "dropout", "embedding_fwd", "embedding_bwd",
+ * "rms_norm_fwd", "rms_norm_bwd", "norm_residual_fwd", "norm_residual_bwd" (each call as a whole).
  * Recording is off by default and costs nothing then.
  */
 int cg_prof_enable(int on);
