@@ -3,48 +3,9 @@
 //   norm_residual  u = alpha scale keep(sigmoid(gate) z rho_z w_post),  r = x + u,  h = r rho_r w_pre
 // and their gradients.  With t = g w and xh = x rho, dx = rho (t - xh mean(t xh)) and dw = sum over rows of g xh.
 // Statistics, sums and everything between a load and the one rounding at a store are float32.
-#include "rows.h"
-#include <limits.h>
+#include "norm_kernels.h"
 
 namespace cg {
-
-constexpr int kNormThreads = 256;
-constexpr int kNormWaves = kNormThreads / kWave;
-
-// Arguments of either operator, forward and backward; rms_norm uses the z side as its input x and leaves the rest
-// at its defaults.
-struct NormArgs {
-  const void *z, *x, *gate, *dr, *dh, *r_in;
-  void *r, *h, *dz, *dx, *dgate;
-  int64_t ldz, ldx, ldgate, lddr, lddh, ldr_in, ldr, ldh, lddz, lddx, lddgate;
-  const void *w_post, *w_pre, *scale;
-  int w_f32, gate_kind;
-  float alpha, eps;
-  float *rstd_z, *rstd_r;  // written forward, read backward
-  float *partial;          // backward: [workgroups][2][d]: columns of q and of dw_pre
-  Mask mask;
-  int64_t n;
-  int32_t d;
-};
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
-}
-// every thread of the workgroup gets the sum; `slots` is rewritten only after everybody has read it
-__device__ __forceinline__ float group_sum(float v, float *slots) {
-  v = wave_sum(v);
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  __syncthreads();
-  if (lane == 0) slots[wave] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int w = 0; w < kNormWaves; ++w) s += slots[w];
-  return s;
-}
-__device__ __forceinline__ float sigmoid(float a) { return 1.f / (1.f + expf(-a)); }
 
 // ---------------------------------------------------------------------------------------------
 // Rows of any length: one workgroup per row, the row read again for every pass over it.
@@ -52,14 +13,15 @@ __device__ __forceinline__ float sigmoid(float a) { return 1.f / (1.f + expf(-a)
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  __shared__ float slots[kNormWaves];
+  __shared__ float slots[2][kNormWaves];
+  int turn = 0;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T *z = (const T *)a.z + row * a.ldz;
     float s = 0.f;
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) s += (float)z[j] * (float)z[j];
-    const float rho_z = 1.f / sqrtf(group_sum(s, slots) / (float)a.d + a.eps);
+    const float rho_z = 1.f / sqrtf(row_sum<kNormThreads>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_z[row] = rho_z;
     if (!RESIDUAL) {
       T *h = (T *)a.h + row * a.ldh;
@@ -82,7 +44,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
       r[j] = (T)v;
       s += v * v;
     }
-    const float rho_r = 1.f / sqrtf(group_sum(s, slots) / (float)a.d + a.eps);
+    const float rho_r = 1.f / sqrtf(row_sum<kNormThreads>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_r[row] = rho_r;
     // h comes from the sum before its rounding to the stored type
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = (T)(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
@@ -94,11 +56,15 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  __shared__ float slots[kNormWaves];
+  __shared__ float slots[2][kNormWaves];
+  int turn = 0;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
-  float *q = a.partial + (int64_t)blockIdx.x * 2 * a.d, *dwp = q + a.d;
-  for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) q[j] = dwp[j] = 0.f;
+  float *q = a.partial + (int64_t)blockIdx.x * (RESIDUAL ? 2 : 1) * a.d, *dwp = q + a.d;
+  for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
+    q[j] = 0.f;
+    if (RESIDUAL) dwp[j] = 0.f;
+  }
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T *z = (const T *)a.z + row * a.ldz;
     const T *dh = a.dh ? (const T *)a.dh + row * a.lddh : nullptr;
@@ -108,7 +74,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       float s = 0.f;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
         s += (float)dh[j] * weight_at<T>(a.w_post, a.w_f32, j) * ((float)z[j] * rho_z);
-      const float m = group_sum(s, slots) / (float)a.d;
+      const float m = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
         const float zh = (float)z[j] * rho_z, g = (float)dh[j];
         q[j] += g * zh;
@@ -125,7 +91,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       float s = 0.f;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
         s += (float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) * ((float)r[j] * rho_r);
-      mean_r = group_sum(s, slots) / (float)a.d;
+      mean_r = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
     }
     auto into = [&](int32_t j) {  // gradient of the residual sum
       float v = dr ? (float)dr[j] : 0.f;
@@ -150,9 +116,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       else if (dgate)
         dgate[j] = (T)dg;
     }
-    const float mean_z = group_sum(s, slots) / (float)a.d;
+    const float mean_z = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
     if (a.gate_kind == CG_GATE_ROW) {
-      sg = group_sum(sg, slots);
+      sg = row_sum<kNormThreads>(sg, slots, turn);
       if (dgate && threadIdx.x == 0) dgate[0] = (T)sg;
     }
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
@@ -163,31 +129,36 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
   }
 }
 
-// dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added in order.  One workgroup per
-// 64 columns; its 4 waves take every fourth slice, then their four sums are added in order.
-template <int DT>
-__global__ __launch_bounds__(kNormThreads) void norm_weight_grads_kernel(NormArgs a, int32_t slices, void *dw_post,
-                                                                         void *dw_pre, void *dscale) {
+// dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added up.  One workgroup per 32
+// columns; 32 threads share a column, each adds every 32nd slice in order, then the 32 sums are added in order.
+constexpr int kFoldCols = 32, kFoldTeams = 32;
+
+template <int DT, bool RESIDUAL>
+__global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kernel(NormArgs a, int32_t slices, void *dw_post,
+                                                                                  void *dw_pre, void *dscale) {
   typedef typename Elem<DT>::type T;
-  __shared__ float sq[kNormWaves][kWave], sp[kNormWaves][kWave];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int32_t j = blockIdx.x * kWave + lane;
+  __shared__ float sq[kFoldTeams][kFoldCols + 1], sp[kFoldTeams][kFoldCols + 1];
+  const int col = threadIdx.x % kFoldCols, team = threadIdx.x / kFoldCols;
+  const int32_t j = blockIdx.x * kFoldCols + col;
+  const int64_t step = (int64_t)(RESIDUAL ? 2 : 1) * a.d;
   float q = 0.f, p = 0.f;
-  if (j < a.d)
-    for (int32_t k = wave; k < slices; k += kNormWaves) {
-      const float *at = a.partial + (int64_t)k * 2 * a.d + j;
+  if (j < a.d) {
+#pragma unroll 4
+    for (int32_t k = team; k < slices; k += kFoldTeams) {
+      const float *at = a.partial + k * step + j;
       q += at[0];
-      p += at[a.d];
+      if (RESIDUAL) p += at[a.d];
     }
-  sq[wave][lane] = q;
-  sp[wave][lane] = p;
+  }
+  sq[team][col] = q;
+  if (RESIDUAL) sp[team][col] = p;
   __syncthreads();
-  if (wave != 0 || j >= a.d) return;
+  if (team != 0 || j >= a.d) return;
   q = p = 0.f;
-#pragma unroll
-  for (int w = 0; w < kNormWaves; ++w) {
-    q += sq[w][lane];
-    p += sp[w][lane];
+#pragma unroll 8
+  for (int t = 0; t < kFoldTeams; ++t) {
+    q += sq[t][col];
+    if (RESIDUAL) p += sp[t][col];
   }
   if (dw_post) weight_put<T>(dw_post, a.w_f32, j, a.alpha * weight_at<T>(a.scale, a.w_f32, j) * q);
   if (dscale) weight_put<T>(dscale, a.w_f32, j, a.alpha * weight_at<T>(a.w_post, a.w_f32, j) * q);
@@ -195,11 +166,23 @@ __global__ __launch_bounds__(kNormThreads) void norm_weight_grads_kernel(NormArg
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-constexpr int64_t kNormMaxGroups = 1024;  // four workgroups per compute unit
-
-static int64_t norm_groups(int64_t n) { return n < kNormMaxGroups ? n : kNormMaxGroups; }
-
-static size_t norm_workspace(int64_t n, int32_t d) { return (size_t)norm_groups(n) * 2 * (size_t)d * sizeof(float); }
+// Workgroups of a gradient = slices of partial sums: four per compute unit, two where a workgroup holds one row at a
+// time (long rows: the slices are as long and the loads of two workgroups keep the memory busy).
+static int64_t norm_groups(int64_t n, int32_t d, int dtype) {
+  const NormShape sh = norm_shape(d, dtype);
+  const int64_t most = sh.lanes == 0 || sh.lanes == kNormThreads ? 512 : 1024;
+  const int64_t want = ceil_div64(n, norm_rows_at_once(sh));
+  return want < most ? want : most;
+}
+// an upper bound for every type and both operators
+static size_t norm_workspace(int64_t n, int32_t d) {
+  int64_t groups = 0;
+  for (int dtype : {CG_F32, CG_BF16}) {
+    const int64_t g = norm_groups(n, d, dtype);
+    groups = g > groups ? g : groups;
+  }
+  return (size_t)groups * 2 * (size_t)d * sizeof(float);
+}
 
 static int check_weights(const char *who, int dtype, int wdtype) {
   if (wdtype != CG_F32 && wdtype != dtype)
@@ -214,7 +197,8 @@ static int check_float(const char *who, const char *what, float v, bool positive
 
 template <bool RESIDUAL>
 static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
-  int64_t groups = a.n < 256 * 32 ? a.n : 256 * 32;
+  if (norm_shape(a.d, dtype).lanes > 0) return launch_norm_fwd(a, RESIDUAL, dtype, s);
+  const int64_t groups = a.n < 256 * 32 ? a.n : 256 * 32;
 #define CG_CALL(DT) norm_fwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
   CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
@@ -224,17 +208,20 @@ static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
 
 template <bool RESIDUAL>
 static int norm_bwd(const NormArgs &a, int dtype, void *dw_post, void *dw_pre, void *dscale, hipStream_t s) {
-  const int64_t groups = norm_groups(a.n);
-  if (groups > 0) {
+  const int64_t groups = norm_groups(a.n, a.d, dtype);
+  if (groups > 0 && norm_shape(a.d, dtype).lanes > 0) {
+    CG_TRY(launch_norm_bwd(a, RESIDUAL, dtype, groups, s));
+  } else if (groups > 0) {
 #define CG_CALL(DT) norm_bwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
     CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
     CG_LAUNCH_CHECK();
   }
   if (dw_post || dw_pre || dscale) {
-#define CG_CALL(DT)                                                                                                   \
-  norm_weight_grads_kernel<DT><<<(unsigned)ceil_div64(a.d, kWave), kNormThreads, 0, s>>>(a, (int32_t)groups, dw_post, \
-                                                                                         dw_pre, dscale)
+    const unsigned cols = (unsigned)ceil_div64(a.d, kFoldCols);
+#define CG_CALL(DT)                                                                                            \
+  norm_weight_grads_kernel<DT, RESIDUAL><<<cols, kFoldCols * kFoldTeams, 0, s>>>(a, (int32_t)groups, dw_post, \
+                                                                                 dw_pre, dscale)
     CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
     CG_LAUNCH_CHECK();

@@ -1,0 +1,245 @@
+// Gradients of rms_norm and norm_residual with the row in registers: every operand is read once and every result
+// written once.  The gradients of the weights are sums over all rows: each lane adds its columns up over the rows its
+// team takes, the teams and wavefronts of a workgroup are added at the end, and one slice per workgroup goes to memory
+// (norm_weight_grads_kernel adds the slices).
+#include "norm_kernels.h"
+
+namespace cg {
+
+// the workgroup's columns of one sum, added over its teams in a fixed order, to dst[0..d)
+template <typename T, int LANES, int K>
+__device__ __forceinline__ void fold_columns(float (&acc)[K][Chunk<T>::V], const Chunk<T> (&c)[K], float *lds,
+                                             float *__restrict__ dst, int32_t d) {
+  constexpr int V = Chunk<T>::V;
+  if (LANES > kWave) {  // every column belongs to one lane
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < c[k].live) dst[((int)threadIdx.x + k * LANES) * V + i] = acc[k][i];
+    return;
+  }
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+      for (int off = LANES; off < kWave; off <<= 1) acc[k][i] += __shfl_xor(acc[k][i], off, kWave);
+      if (lane < LANES) lds[wave * (LANES * K * V) + (lane + k * LANES) * V + i] = acc[k][i];
+    }
+  __syncthreads();
+  for (int j = threadIdx.x; j < d; j += kNormThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNormWaves; ++w) s += lds[w * (LANES * K * V) + j];
+    dst[j] = s;
+  }
+  __syncthreads();
+}
+
+template <int DT, int LANES, int K, bool RESIDUAL>
+__global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
+  typedef typename Elem<DT>::type T;
+  typedef Chunk<T> C;
+  constexpr int V = C::V, TEAMS = kNormThreads / LANES;
+  __shared__ float slots[2][kNormWaves];
+  __shared__ float lds[LANES > kWave ? 1 : kNormWaves * LANES * K * V];
+  int turn = 0;
+  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  C c[K];
+  float wz[K][V], wr[K][V], q[K][V], p[K][V];  // alpha scale w_post (w_post alone for rms_norm), w_pre, column sums
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int32_t j = (lane + k * LANES) * V;
+    c[k].place(j, a.d);
+    weight_chunk<T>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
+    if (RESIDUAL) {
+      float s[V];
+      weight_chunk<T>(a.scale, a.w_f32, j, c[k].live, s);
+      weight_chunk<T>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) wz[k][i] *= a.alpha * s[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[k][i] = p[k][i] = 0.f;
+  }
+  const float inv_d = 1.f / (float)a.d;
+  MaskKey key = {0, 0, 0, 0};
+  if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
+  const int64_t step = (int64_t)gridDim.x * TEAMS;
+  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < a.n; row += step) {
+    Raw rz[K], rdh[K], rr[K], rdr[K], rg[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) rz[k] = c[k].load((const T *)a.z + row * a.ldz);
+    if (!RESIDUAL || a.dh) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) rdh[k] = c[k].load((const T *)a.dh + row * a.lddh);
+    }
+    const float rho_z = a.rstd_z[row];
+    if (!RESIDUAL) {
+      float zh[K][V], t[K][V], s = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        c[k].floats(rz[k], zh[k]);
+        c[k].floats(rdh[k], t[k]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          zh[k][i] *= rho_z;
+          q[k][i] += t[k][i] * zh[k][i];
+          t[k][i] *= wz[k][i];
+          s += t[k][i] * zh[k][i];
+        }
+      }
+      const float m = row_sum<LANES>(s, slots, turn) * inv_d;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[k][i] = rho_z * (t[k][i] - zh[k][i] * m);
+        c[k].write((T *)a.dz + row * a.lddz, t[k]);
+      }
+      continue;
+    }
+    if (a.dh) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) rr[k] = c[k].load((const T *)a.r_in + row * a.ldr_in);
+    }
+    if (a.dr) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) rdr[k] = c[k].load((const T *)a.dr + row * a.lddr);
+    }
+    float row_gate = 0.f;
+    if (a.gate_kind == CG_GATE_FULL) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) rg[k] = c[k].load((const T *)a.gate + row * a.ldgate);
+    } else if (a.gate_kind == CG_GATE_ROW) {
+      row_gate = (float)((const T *)a.gate)[row * a.ldgate];
+    }
+    float D[K][V], zh[K][V];  // gradient of the residual sum; the normalised block output
+    if (a.dh) {
+      const float rho_r = a.rstd_r[row];
+      float rh[K][V], s = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        c[k].floats(rdh[k], D[k]);
+        c[k].floats(rr[k], rh[k]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          rh[k][i] *= rho_r;
+          p[k][i] += D[k][i] * rh[k][i];
+          D[k][i] *= wr[k][i];
+          s += D[k][i] * rh[k][i];
+        }
+      }
+      const float m = row_sum<LANES>(s, slots, turn) * inv_d;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[k][i] = rho_r * (D[k][i] - rh[k][i] * m);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[k][i] = 0.f;
+    }
+    if (a.dr) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float g[V];
+        c[k].floats(rdr[k], g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[k][i] += g[i];
+      }
+    }
+    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid(row_gate) : 1.f;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      c[k].write((T *)a.dx + row * a.lddx, D[k]);
+      c[k].floats(rz[k], zh[k]);
+      if (a.mask.rng) {
+        float m[V];
+        mask_chunk<V>(key, a.mask, row, (lane + k * LANES) * V, m);
+#pragma unroll
+        for (int i = 0; i < V; ++i) D[k][i] = m[i] > 0.f ? D[k][i] * m[i] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) zh[k][i] *= rho_z;
+      if (a.gate_kind == CG_GATE_FULL) {
+        float g[V];
+        c[k].floats(rg[k], g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float sig = sigmoid(g[i]), e = D[k][i] * wz[k][i];
+          q[k][i] += D[k][i] * sig * zh[k][i];
+          g[i] = e * zh[k][i] * (sig * (1.f - sig));
+          D[k][i] = e * sig;
+        }
+        c[k].write((T *)a.dgate + row * a.lddgate, g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          q[k][i] += D[k][i] * row_sig * zh[k][i];
+          D[k][i] *= wz[k][i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) s += D[k][i] * zh[k][i];
+    }
+    s = row_sum<LANES>(s, slots, turn);
+    if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = (T)(s * (row_sig * (1.f - row_sig)));
+    const float m = s * inv_d, rho_s = rho_z * row_sig;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) D[k][i] = rho_s * (D[k][i] - zh[k][i] * m);
+      c[k].write((T *)a.dz + row * a.lddz, D[k]);
+    }
+  }
+  float *slice = a.partial + (int64_t)blockIdx.x * (RESIDUAL ? 2 : 1) * a.d;
+  fold_columns<T, LANES, K>(q, c, lds, slice, a.d);
+  if (RESIDUAL) fold_columns<T, LANES, K>(p, c, lds, slice + a.d, a.d);
+}
+
+template <int DT, int LANES, int K>
+static int go(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
+  if (residual)
+    norm_bwd_kernel<DT, LANES, K, true><<<(unsigned)groups, kNormThreads, 0, s>>>(a);
+  else
+    norm_bwd_kernel<DT, LANES, K, false><<<(unsigned)groups, kNormThreads, 0, s>>>(a);
+  CG_LAUNCH_CHECK();
+  return CG_OK;
+}
+
+template <int DT>
+static int go_shape(const NormArgs &a, bool residual, const NormShape &sh, int64_t n, hipStream_t s) {
+  constexpr bool F32 = DT == CG_F32;
+  switch (sh.lanes * 16 + sh.chunks) {
+    case 4 * 16 + 1: return go<DT, 4, 1>(a, residual, n, s);
+    case 8 * 16 + 1: return go<DT, 8, 1>(a, residual, n, s);
+    case 16 * 16 + 1: return go<DT, 16, 1>(a, residual, n, s);
+    case 32 * 16 + 1: return go<DT, 32, 1>(a, residual, n, s);
+    case 64 * 16 + 1: return go<DT, 64, 1>(a, residual, n, s);
+    case 64 * 16 + 2: return go<DT, 64, 2>(a, residual, n, s);
+    case 64 * 16 + 3: if (F32) return go<DT, 64, F32 ? 3 : 1>(a, residual, n, s); break;
+    case 64 * 16 + 4: if (F32) return go<DT, 64, F32 ? 4 : 1>(a, residual, n, s); break;
+    case 256 * 16 + 1: if (!F32) return go<DT, 256, 1>(a, residual, n, s); break;
+    case 256 * 16 + 2: return go<DT, 256, 2>(a, residual, n, s);
+    case 256 * 16 + 3: return go<DT, 256, 3>(a, residual, n, s);
+    case 256 * 16 + 4: return go<DT, 256, 4>(a, residual, n, s);
+    case 256 * 16 + 5: if (F32) return go<DT, 256, F32 ? 5 : 2>(a, residual, n, s); break;
+    case 256 * 16 + 6: if (F32) return go<DT, 256, F32 ? 6 : 2>(a, residual, n, s); break;
+    case 256 * 16 + 7: if (F32) return go<DT, 256, F32 ? 7 : 2>(a, residual, n, s); break;
+    case 256 * 16 + 8: if (F32) return go<DT, 256, F32 ? 8 : 2>(a, residual, n, s); break;
+  }
+  CG_FAIL(CG_ERR_UNSUPPORTED, "norm: no kernel for %d lanes of %d chunks", sh.lanes, sh.chunks);
+}
+
+int launch_norm_bwd(const NormArgs &a, bool residual, int dtype, int64_t groups, hipStream_t s) {
+  const NormShape sh = norm_shape(a.d, dtype);
+  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, sh, groups, s);
+  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, sh, groups, s);
+  return go_shape<CG_F16>(a, residual, sh, groups, s);
+}
+
+}  // namespace cg

@@ -1,0 +1,92 @@
+// Arguments, reductions and the choice of lanes per row of the norm kernels (norm.hip, norm_fwd.hip, norm_bwd.hip).
+#pragma once
+#include "rows.h"
+
+namespace cg {
+
+constexpr int kNormThreads = 256;
+constexpr int kNormWaves = kNormThreads / kWave;
+
+// Arguments of either operator, forward and backward; rms_norm uses the z side as its input x and leaves the rest
+// at its defaults.
+struct NormArgs {
+  const void *z, *x, *gate, *dr, *dh, *r_in;
+  void *r, *h, *dz, *dx, *dgate;
+  int64_t ldz, ldx, ldgate, lddr, lddh, ldr_in, ldr, ldh, lddz, lddx, lddgate;
+  const void *w_post, *w_pre, *scale;
+  int w_f32, gate_kind;
+  float alpha, eps;
+  float *rstd_z, *rstd_r;  // written forward, read backward
+  float *partial;          // backward: one slice per workgroup, [d] of q and for the residual block [d] of dw_pre
+  Mask mask;
+  int64_t n;
+  int32_t d;
+};
+
+// Lanes that share a row and 16-byte chunks each of them holds.  Rows of up to 64 chunks are taken by the smallest
+// power of two of lanes (at least 4) that covers them with one chunk each, several rows per wavefront; longer rows by a
+// whole wavefront with up to 16 elements a lane; then by a workgroup of 256 lanes with up to 32 elements a lane.
+// lanes == 0: the row does not fit and is read again for every pass over it.
+struct NormShape {
+  int lanes, chunks;
+};
+static inline NormShape norm_shape(int32_t d, int dtype) {
+  const int v = dtype == CG_F32 ? 4 : 8;
+  const int64_t c = ceil_div64(d, v);
+  if (c <= kWave) {
+    int lanes = 4;
+    while (lanes < c) lanes *= 2;
+    return NormShape{lanes, 1};
+  }
+  if (c <= (int64_t)kWave * (16 / v)) return NormShape{kWave, (int)ceil_div64(c, kWave)};
+  if (c <= (int64_t)kNormThreads * (32 / v)) return NormShape{kNormThreads, (int)ceil_div64(c, kNormThreads)};
+  return NormShape{0, 0};
+}
+static inline int norm_rows_at_once(const NormShape &s) {
+  return s.lanes == 0 || s.lanes == kNormThreads ? 1 : kNormThreads / s.lanes;
+}
+
+int launch_norm_fwd(const NormArgs &a, bool residual, int dtype, hipStream_t s);
+int launch_norm_bwd(const NormArgs &a, bool residual, int dtype, int64_t groups, hipStream_t s);
+
+// Sum over the lanes of a row.  Teams inside a wavefront exchange registers; a whole workgroup goes through `slots`,
+// whose halves alternate from one reduction to the next, so that one barrier a reduction is enough: a half is written
+// again only after everybody has passed the barrier of the reduction in between, hence has read it.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float (*slots)[kNormWaves], int &turn) {
+#pragma unroll
+  for (int off = (LANES < kWave ? LANES : kWave) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if (LANES <= kWave) return v;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  if (lane == 0) slots[turn][wave] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < kNormWaves; ++w) s += slots[turn][w];
+  turn ^= 1;
+  return s;
+}
+
+// v_rcp_f32 and v_rsq_f32 are within one unit of the last place; exp's argument is exact
+__device__ __forceinline__ float sigmoid(float a) { return __builtin_amdgcn_rcpf(1.f + expf(-a)); }
+
+// a weight vector's elements of one chunk, ones for a null pointer, zeros behind the row's end
+template <typename T>
+__device__ __forceinline__ void weight_chunk(const void *w, int w_f32, int32_t j, int live, float (&out)[Chunk<T>::V]) {
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::V; ++i) out[i] = i < live ? weight_at<T>(w, w_f32, j + i) : 0.f;
+}
+
+// 1 / (1 - p) or 0 for the elements of the chunk that starts at column j (a multiple of four)
+template <int V>
+__device__ __forceinline__ void mask_chunk(const MaskKey &k, const Mask &m, int64_t row, int32_t j, float (&out)[V]) {
+#pragma unroll
+  for (int b = 0; b < V / 4; ++b) {
+    uint32_t w[4];
+    mask_words(k, (uint32_t)row, (uint32_t)(j / 4 + b), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[4 * b + i] = w[i] > m.last ? m.inv_keep : 0.f;
+  }
+}
+
+}  // namespace cg
