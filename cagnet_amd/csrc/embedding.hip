@@ -19,31 +19,49 @@ __device__ __forceinline__ int64_t index_at(const IndexView &v, int64_t i) {
   return v.wide ? static_cast<const int64_t *>(v.idx)[i] : (int64_t) static_cast<const int32_t *>(v.idx)[i];
 }
 
+// Lanes that share a row: a power of two that covers its 16-byte chunks, at most a workgroup (longer rows are taken in
+// strides of it); lanes beyond the row's end have nothing to do.
+static inline int lanes_log2(int32_t d, int per_chunk) {
+  const int64_t c = ceil_div64(d, per_chunk);
+  int log2 = 0;
+  while (((int64_t)1 << log2) < c && log2 < 8) ++log2;
+  return log2;
+}
+
 // ---------------------------------------------------------------------------------------------
-// lookup: one wave per position and 16 bytes per lane
+// lookup: kLookups rows a team at once, all indices loaded before the first row and all rows before the first store
 // ---------------------------------------------------------------------------------------------
+constexpr int kLookups = 4;
+
 template <int DT>
 __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typename Elem<DT>::type *__restrict__ table,
                                                                     int64_t ldt, int64_t rows, IndexView idx, int64_t n,
-                                                                    int32_t d, float scale,
+                                                                    int32_t d, float scale, int lanes_log,
                                                                     typename Elem<DT>::type *__restrict__ out,
                                                                     int64_t ldo) {
   typedef typename Elem<DT>::type T;
-  constexpr int V = 16 / sizeof(T);
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t waves = (int64_t)gridDim.x * kEmbWaves;
-  for (int64_t i = (int64_t)blockIdx.x * kEmbWaves + threadIdx.x / kWave; i < n; i += waves) {
-    const int64_t v = index_at(idx, i);
-    const bool in = v >= 0 && v < rows;
-    const T *src = table + (in ? v : 0) * ldt;
-    T *dst = out + i * ldo;
-    for (int32_t j = lane * V; j < d; j += kWave * V) {
-      const int live = d - j < V ? d - j : V;
-      float f[V];
-      load_some(src + j, in ? live : 0, f);
+  typedef Chunk<T> C;
+  const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
+  const int64_t step = (int64_t)gridDim.x * teams * kLookups;
+  for (int64_t i0 = ((int64_t)blockIdx.x * teams + (threadIdx.x >> lanes_log)) * kLookups; i0 < n; i0 += step) {
+    int64_t v[kLookups];
 #pragma unroll
-      for (int k = 0; k < V; ++k) f[k] = in ? f[k] * scale : 0.f;
-      store_some(dst + j, live, f);
+    for (int k = 0; k < kLookups; ++k) v[k] = index_at(idx, i0 + k < n ? i0 + k : n - 1);
+    for (int32_t j = lane * C::V; j < d; j += lanes * C::V) {
+      C c;
+      c.place(j, d);
+      Raw r[kLookups];
+#pragma unroll
+      for (int k = 0; k < kLookups; ++k) r[k] = c.load(table + (v[k] >= 0 && v[k] < rows ? v[k] : 0) * ldt);
+#pragma unroll
+      for (int k = 0; k < kLookups; ++k) {
+        float f[C::V];
+        c.floats(r[k], f);
+        const bool in = v[k] >= 0 && v[k] < rows;
+#pragma unroll
+        for (int i = 0; i < C::V; ++i) f[i] = in ? f[i] * scale : 0.f;
+        if (i0 + k < n) c.write(out + (i0 + k) * ldo, f);
+      }
     }
   }
 }
@@ -218,55 +236,172 @@ __global__ __launch_bounds__(kEmbThreads) void emb_scatter_kernel(KeySource src,
 }
 
 // ---------------------------------------------------------------------------------------------
-// sums: one wave per table row adds the rows of g that its segment of sorted positions names
+// Sums.  rowptr[v] .. rowptr[v + 1] are the sorted positions of table row v.  A row with up to `span` of them is added
+// up by one team of lanes.  The sorted array is also cut into chunks of `span` positions: a row with more than `span`
+// ("hot": with popular indices one row can hold a tenth of all) covers the end of at least one chunk, so a chunk holds a
+// part of at most two hot rows, the one it begins in and the one it ends in.  A team adds up each part into a partial
+// row, and a second kernel adds a hot row's partial rows in order.
 // ---------------------------------------------------------------------------------------------
+struct SumArgs {
+  const void *g;
+  int64_t ldg;
+  const int32_t *rowptr, *key, *pos;
+  int64_t rows;
+  int32_t n, d, span;
+  float scale, beta;
+  void *out;
+  int64_t ldo;
+  float *partial;  // [2 * chunks][d], float32
+  unsigned chunk_groups, chunk_teams;
+};
+
+constexpr int kAhead = 4;  // rows of g in flight per lane
+
+// the chunk's columns of g's rows pos[from .. to), added in order
+template <typename T>
+__device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T> &c, int32_t from, int32_t to,
+                                         float (&sum)[Chunk<T>::V]) {
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::V; ++i) sum[i] = 0.f;
+  for (int32_t at = from; at < to; at += kAhead) {
+    int32_t p[kAhead];
+    Raw r[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) p[k] = a.pos[at + k < to ? at + k : to - 1];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) r[k] = c.load((const T *)a.g + (int64_t)p[k] * a.ldg);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float f[Chunk<T>::V];
+      c.floats(r[k], f);
+#pragma unroll
+      for (int i = 0; i < Chunk<T>::V; ++i) sum[i] += at + k < to ? f[i] : 0.f;
+    }
+  }
+}
+
 template <int DT, bool OUT_F32>
-__global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(const typename Elem<DT>::type *__restrict__ g, int64_t ldg,
-                                                              const int32_t *__restrict__ rowptr,
-                                                              const int32_t *__restrict__ pos, int64_t rows, int32_t d,
-                                                              float scale, float beta, void *__restrict__ out_,
-                                                              int64_t ldo) {
+__global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lanes_log) {
   typedef typename Elem<DT>::type T;
   typedef typename Elem<OUT_F32 ? CG_F32 : DT>::type O;
-  constexpr int V = 16 / sizeof(T);
-  O *out = static_cast<O *>(out_);
-  const int lane = threadIdx.x & (kWave - 1);
-  const int64_t waves = (int64_t)gridDim.x * kEmbWaves;
-  for (int64_t v = (int64_t)blockIdx.x * kEmbWaves + threadIdx.x / kWave; v < rows; v += waves) {
-    const int32_t from = rowptr[v], to = rowptr[v + 1];
-    if (from == to && beta == 1.f) continue;
-    for (int32_t j = lane * V; j < d; j += kWave * V) {
-      const int live = d - j < V ? d - j : V;
-      float sum[V];
+  constexpr int V = Chunk<T>::V;
+  const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
+  const int team = threadIdx.x >> lanes_log;
+  if (blockIdx.x < a.chunk_groups) {  // parts of hot rows
+    const int32_t chunk = (int32_t)blockIdx.x * teams + team;
+    if (chunk >= (int32_t)a.chunk_teams) return;
+    const int32_t all = a.rowptr[a.rows], begin = chunk * a.span;
+    if (begin >= all) return;
+    const int32_t end = all - begin < a.span ? all : begin + a.span;
+    const int32_t first = a.key[begin], last = a.key[end - 1];
 #pragma unroll
-      for (int k = 0; k < V; ++k) sum[k] = 0.f;
-      for (int32_t i = from; i < to; ++i) {
-        float f[V];
-        load_some(g + (int64_t)pos[i] * ldg + j, live, f);
-#pragma unroll
-        for (int k = 0; k < V; ++k) sum[k] += f[k];
+    for (int part = 0; part < 2; ++part) {
+      const int32_t v = part == 0 ? first : last, from = a.rowptr[v], to = a.rowptr[v + 1];
+      if (to - from <= a.span || (part == 1 && first == last)) continue;
+      float *dst = a.partial + ((int64_t)chunk * 2 + part) * a.d;
+      for (int32_t j = lane * V; j < a.d; j += lanes * V) {
+        Chunk<T> c;
+        c.place(j, a.d);
+        float sum[V];
+        add_rows<T>(a, c, from > begin ? from : begin, to < end ? to : end, sum);
+        store_some<float, V>(dst + j, c.live, sum);
       }
-      float old[V];
-      if (beta != 0.f) load_some(out + v * ldo + j, live, old);
-#pragma unroll
-      for (int k = 0; k < V; ++k) sum[k] = beta != 0.f ? sum[k] * scale + beta * old[k] : sum[k] * scale;
-      store_some(out + v * ldo + j, live, sum);
     }
+    return;
+  }
+  const int64_t step = (int64_t)(gridDim.x - a.chunk_groups) * teams;
+  for (int64_t v = (int64_t)(blockIdx.x - a.chunk_groups) * teams + team; v < a.rows; v += step) {
+    const int32_t from = a.rowptr[v], to = a.rowptr[v + 1];
+    if (to - from > a.span || (from == to && a.beta == 1.f)) continue;
+    O *out = (O *)a.out + v * a.ldo;
+    for (int32_t j = lane * V; j < a.d; j += lanes * V) {
+      Chunk<T> c;
+      c.place(j, a.d);
+      float sum[V];
+      add_rows<T>(a, c, from, to, sum);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] *= a.scale;
+      if (a.beta != 0.f) {
+        float old[V];
+        load_some<O, V>(out + j, c.live, old);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += a.beta * old[i];
+      }
+      store_some<O, V>(out + j, c.live, sum);
+    }
+  }
+}
+
+// One workgroup per chunk and 256 columns; it has work if a hot row begins in its chunk (at most one does: it covers
+// the chunk's end).  Its 16 waves take every 16th partial row each, their sums are added in order.
+constexpr int kFoldWaves = 16, kFoldColumns = kWave * 4;
+
+template <int OT>
+__global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) {
+  typedef typename Elem<OT>::type O;
+  __shared__ float lds[kFoldWaves][kFoldColumns];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int32_t j = blockIdx.y * kFoldColumns + lane * 4, all = a.rowptr[a.rows];
+  Chunk<float> c;
+  c.place(j, a.d);
+  for (int32_t chunk = blockIdx.x; chunk < (int32_t)a.chunk_teams; chunk += gridDim.x) {  // uniform in the workgroup
+    const int32_t begin = chunk * a.span;
+    if (begin >= all) return;
+    const int32_t end = all - begin < a.span ? all : begin + a.span;
+    const int32_t v = a.key[end - 1], from = a.rowptr[v], to = a.rowptr[v + 1];
+    if (to - from <= a.span || from < begin) continue;
+    const int32_t chunks = (to - 1) / a.span - chunk + 1;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c.live > 0) {
+#pragma unroll 4
+      for (int32_t k = wave; k < chunks; k += kFoldWaves) {
+        // the row's part in its first chunk is that chunk's last part unless the chunk begins with it
+        const int64_t slot = (int64_t)(chunk + k) * 2 + (k == 0 && from > begin ? 1 : 0);
+        float f[4];
+        load_some<float, 4>(a.partial + slot * a.d + j, c.live, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += f[i];
+      }
+    }
+    __syncthreads();  // the sums of the chunk before have been read
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[wave][lane * 4 + i] = sum[i];
+    __syncthreads();
+    if (wave != 0 || c.live <= 0) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum[i] = 0.f;
+      for (int w = 0; w < kFoldWaves; ++w) sum[i] += lds[w][lane * 4 + i];
+      sum[i] *= a.scale;
+    }
+    O *out = (O *)a.out + v * a.ldo;
+    if (a.beta != 0.f) {
+      float old[4];
+      load_some<O, 4>(out + j, c.live, old);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] += a.beta * old[i];
+    }
+    store_some<O, 4>(out + j, c.live, sum);
   }
 }
 
 // ---- host side ------------------------------------------------------------------------------------
 struct EmbPlan {
   int passes, dbits;
-  int64_t tiles;
-  size_t key[2], pos[2], hist, totals, rowptr, bytes;  // offsets into the workspace
+  int64_t tiles, chunks;
+  int32_t span;
+  size_t key[2], pos[2], hist, totals, rowptr, partial, bytes;  // offsets into the workspace
 };
-static EmbPlan emb_plan(int64_t n, int64_t rows) {
+static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   EmbPlan p = {};
   int bits = bits_for((int32_t)(rows + 1));
   p.passes = bits > 0 ? (bits + kMaxDigit - 1) / kMaxDigit : 1;
   p.dbits = bits > 0 ? (bits + p.passes - 1) / p.passes : 1;
   p.tiles = ceil_div64(n, kEmbTile);
+  // about sqrt(n) / 4: the longest chain of additions in a team and the longest list of partial rows grow alike
+  p.span = 32;
+  while (p.span < 512 && (int64_t)p.span * p.span * 16 < n) p.span *= 2;
+  p.chunks = ceil_div64(n, p.span);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -277,6 +412,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows) {
   p.hist = take((size_t)p.tiles * ((size_t)1 << p.dbits) * 4);
   p.totals = take((size_t)kMaxRadix * 4);
   p.rowptr = take((size_t)(rows + 2) * 4);
+  p.partial = take((size_t)p.chunks * 2 * (size_t)d * 4);
   p.bytes = at;
   return p;
 }
@@ -284,7 +420,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows) {
 static int check_lookup(const char *who, int64_t n, int64_t rows, int32_t d) {
   if (n < 0 || rows <= 0 || d <= 0)
     CG_FAIL(CG_ERR_SIZE, "%s: n=%lld indices into rows=%lld of d=%d elements", who, (long long)n, (long long)rows, d);
-  if (n > 0x7ffffffeLL || rows > 0x7ffffffdLL)
+  if (n > 0x7fff0000LL || rows > 0x7ffffffdLL)
     CG_FAIL(CG_ERR_OVERFLOW, "%s: n=%lld, rows=%lld overflow int32 positions", who, (long long)n, (long long)rows);
   return CG_OK;
 }
@@ -305,12 +441,13 @@ int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void 
   if (d_out == d_table) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the table", who);
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof("embedding_fwd", d, s);
-  int64_t groups = ceil_div64(n, kEmbWaves);
+  const int lanes_log = lanes_log2(d, dtype == CG_F32 ? 4 : 8);
+  int64_t groups = ceil_div64(n, (int64_t)(kEmbThreads >> lanes_log) * kLookups);
   if (groups > 256 * 64) groups = 256 * 64;
   const IndexView view = {d_idx, idx64 != 0};
 #define CG_CALL(DT)                                                                                              \
   embedding_fwd_kernel<DT><<<(unsigned)groups, kEmbThreads, 0, s>>>((const Elem<DT>::type *)d_table, ldt, rows, view, n, \
-                                                                     d, scale, (Elem<DT>::type *)d_out, ldo)
+                                                                     d, scale, lanes_log, (Elem<DT>::type *)d_out, ldo)
   CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();
@@ -321,7 +458,7 @@ int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *byte
   using namespace cg;
   if (!bytes) CG_FAIL(CG_ERR_NULL, "cg_embedding_bwd_workspace: null pointer");
   CG_TRY(check_lookup("cg_embedding_bwd_workspace", n, rows, d));
-  *bytes = (int64_t)emb_plan(n, rows).bytes;
+  *bytes = (int64_t)emb_plan(n, rows, d).bytes;
   return CG_OK;
 }
 
@@ -337,7 +474,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   if (!d_out || !d_work || (n > 0 && (!d_g || !d_idx))) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
   if (ldo < d || (n > 0 && ldg < d)) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
   if (d_out == d_g) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the input", who);
-  const EmbPlan p = emb_plan(n, rows);
+  const EmbPlan p = emb_plan(n, rows, d);
   if (work_bytes < (int64_t)p.bytes) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)p.bytes);
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof("embedding_bwd", d, s);
@@ -362,16 +499,26 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
     }
   }
   CG_TRY(launch_rowptr(key[last], n, (int32_t)(rows + 1), rowptr, s));
-  int64_t groups = ceil_div64(rows, kEmbWaves);
+  const int lanes_log = lanes_log2(d, dtype == CG_F32 ? 4 : 8), teams = kEmbThreads >> lanes_log;
+  SumArgs a = {};
+  a.g = d_g, a.ldg = ldg, a.rowptr = rowptr, a.key = key[last], a.pos = pos[last], a.rows = rows, a.n = (int32_t)n, a.d = d;
+  a.span = p.span, a.scale = scale, a.beta = beta, a.out = d_out, a.ldo = ldo, a.partial = (float *)(w + p.partial);
+  a.chunk_teams = (unsigned)p.chunks, a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
+  int64_t groups = ceil_div64(rows, teams);
   if (groups > 256 * 64) groups = 256 * 64;
-#define CG_CALL(DT)                                                                                                     \
-  if (out_dtype == CG_F32)                                                                                              \
-    emb_sum_kernel<DT, true><<<(unsigned)groups, kEmbThreads, 0, s>>>((const Elem<DT>::type *)d_g, ldg, rowptr, pos[last], \
-                                                                       rows, d, scale, beta, d_out, ldo);               \
-  else                                                                                                                  \
-    emb_sum_kernel<DT, false><<<(unsigned)groups, kEmbThreads, 0, s>>>((const Elem<DT>::type *)d_g, ldg, rowptr, pos[last], \
-                                                                        rows, d, scale, beta, d_out, ldo)
+  groups += a.chunk_groups;
+#define CG_CALL(DT)                                                                  \
+  if (out_dtype == CG_F32)                                                           \
+    emb_sum_kernel<DT, true><<<(unsigned)groups, kEmbThreads, 0, s>>>(a, lanes_log); \
+  else                                                                               \
+    emb_sum_kernel<DT, false><<<(unsigned)groups, kEmbThreads, 0, s>>>(a, lanes_log)
   CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_CALL
+  CG_LAUNCH_CHECK();
+  if (n <= p.span) return CG_OK;  // no row can be hot
+  const dim3 fold((unsigned)(p.chunks < 65536 ? p.chunks : 65536), (unsigned)ceil_div64(d, kFoldColumns));
+#define CG_CALL(OT) emb_fold_kernel<OT><<<fold, kWave * kFoldWaves, 0, s>>>(a)
+  CG_BY_DTYPE(out_dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();
   return CG_OK;

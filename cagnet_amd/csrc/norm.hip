@@ -26,7 +26,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
     if (!RESIDUAL) {
       T *h = (T *)a.h + row * a.ldh;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
-        h[j] = (T)((float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j));
+        h[j] = rounded<T>((float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j));
       continue;
     }
     const T *x = (const T *)a.x + row * a.ldx;
@@ -41,13 +41,13 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
     T *r = (T *)a.r + row * a.ldr, *h = (T *)a.h + row * a.ldh;
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
       const float v = sum_at(j);
-      r[j] = (T)v;
+      r[j] = rounded<T>(v);
       s += v * v;
     }
     const float rho_r = 1.f / sqrtf(row_sum<kNormThreads>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_r[row] = rho_r;
     // h comes from the sum before its rounding to the stored type
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = (T)(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
+    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = rounded<T>(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
   }
 }
 
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
         const float zh = (float)z[j] * rho_z, g = (float)dh[j];
         q[j] += g * zh;
-        dz[j] = (T)(rho_z * (g * weight_at<T>(a.w_post, a.w_f32, j) - zh * m));
+        dz[j] = rounded<T>(rho_z * (g * weight_at<T>(a.w_post, a.w_f32, j) - zh * m));
       }
       continue;
     }
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
       const float D = into(j), zh = (float)z[j] * rho_z, sig = gate_at(j), Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
       const float e = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j);
-      dx[j] = (T)D;
+      dx[j] = rounded<T>(D);
       s += e * sig * zh;
       q[j] += Dm * sig * zh;
       if (dh) dwp[j] += (float)dh[j] * ((float)r[j] * rho_r);
@@ -114,17 +114,17 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       if (a.gate_kind == CG_GATE_ROW)
         sg += dg;
       else if (dgate)
-        dgate[j] = (T)dg;
+        dgate[j] = rounded<T>(dg);
     }
     const float mean_z = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
     if (a.gate_kind == CG_GATE_ROW) {
       sg = row_sum<kNormThreads>(sg, slots, turn);
-      if (dgate && threadIdx.x == 0) dgate[0] = (T)sg;
+      if (dgate && threadIdx.x == 0) dgate[0] = rounded<T>(sg);
     }
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
       const float D = into(j), zh = (float)z[j] * rho_z, Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
       const float f = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j) * gate_at(j);
-      dz[j] = (T)(rho_z * (f - zh * mean_z));
+      dz[j] = rounded<T>(rho_z * (f - zh * mean_z));
     }
   }
 }

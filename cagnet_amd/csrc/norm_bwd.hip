@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
       for (int i = 0; i < V; ++i) s += D[k][i] * zh[k][i];
     }
     s = row_sum<LANES>(s, slots, turn);
-    if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = (T)(s * (row_sig * (1.f - row_sig)));
+    if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));
     const float m = s * inv_d, rho_s = rho_z * row_sig;
 #pragma unroll
     for (int k = 0; k < K; ++k) {

@@ -20,6 +20,15 @@ struct Elem<CG_F16> {
   typedef _Float16 type;
 };
 
+// The rounding at a store.  A product that is rounded to float16 right away would be compiled to one instruction that
+// rounds the exact product once, in some kernels and not in others; held in a register in between, it is float32
+// arithmetic and then a rounding everywhere, for every type.
+template <typename T>
+__device__ __forceinline__ T rounded(float v) {
+  if (sizeof(T) == 2) asm("" : "+v"(v));
+  return (T)v;
+}
+
 // N consecutive elements that are only aligned as single elements are: rows of 602 floats start 8 bytes apart from a
 // 16-byte boundary, rows of 41 start anywhere.  The memory pipeline takes wide accesses at any element address, so
 // such rows are moved 16 bytes per lane like aligned ones.
@@ -38,7 +47,7 @@ template <typename T, int N>
 __device__ __forceinline__ void store_pack(T *__restrict__ p, const float (&in)[N]) {
   typename Pack<T, N>::type q;
 #pragma unroll
-  for (int i = 0; i < N; ++i) q[i] = (T)in[i];
+  for (int i = 0; i < N; ++i) q[i] = rounded<T>(in[i]);
   *reinterpret_cast<typename Pack<T, N>::type *>(p) = q;
 }
 // the first `live` (0..N) of N elements; the others read as zero and are not written
@@ -58,7 +67,7 @@ __device__ __forceinline__ void store_some(T *__restrict__ p, int live, const fl
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i < live) p[i] = (T)in[i];
+      if (i < live) p[i] = rounded<T>(in[i]);
   }
 }
 
@@ -119,7 +128,7 @@ struct Chunk {
   __device__ __forceinline__ void write(T *row, const float (&in)[V]) const {
     vec q = {};
 #pragma unroll
-    for (int i = 0; i < V; ++i) q[i] = (T)in[i];
+    for (int i = 0; i < V; ++i) q[i] = rounded<T>(in[i]);
     if (live == V) {
       *reinterpret_cast<vec *>(row + at) = q;
     } else if (live > 0) {
