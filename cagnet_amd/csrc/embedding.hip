@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typena
                                                                     typename Elem<DT>::type *__restrict__ out,
                                                                     int64_t ldo) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T> C;
+  typedef Chunk<T, true> C;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
   const int64_t step = (int64_t)gridDim.x * teams * kLookups;
   for (int64_t i0 = ((int64_t)blockIdx.x * teams + (threadIdx.x >> lanes_log)) * kLookups; i0 < n; i0 += step) {
@@ -259,10 +259,10 @@ constexpr int kAhead = 4;  // rows of g in flight per lane
 
 // the chunk's columns of g's rows pos[from .. to), added in order
 template <typename T>
-__device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T> &c, int32_t from, int32_t to,
-                                         float (&sum)[Chunk<T>::V]) {
+__device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T, true> &c, int32_t from, int32_t to,
+                                         float (&sum)[Chunk<T, true>::V]) {
 #pragma unroll
-  for (int i = 0; i < Chunk<T>::V; ++i) sum[i] = 0.f;
+  for (int i = 0; i < Chunk<T, true>::V; ++i) sum[i] = 0.f;
   for (int32_t at = from; at < to; at += kAhead) {
     int32_t p[kAhead];
     Raw r[kAhead];
@@ -272,10 +272,10 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T> &c, in
     for (int k = 0; k < kAhead; ++k) r[k] = c.load((const T *)a.g + (int64_t)p[k] * a.ldg);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      float f[Chunk<T>::V];
+      float f[Chunk<T, true>::V];
       c.floats(r[k], f);
 #pragma unroll
-      for (int i = 0; i < Chunk<T>::V; ++i) sum[i] += at + k < to ? f[i] : 0.f;
+      for (int i = 0; i < Chunk<T, true>::V; ++i) sum[i] += at + k < to ? f[i] : 0.f;
     }
   }
 }
@@ -284,7 +284,7 @@ template <int DT, bool OUT_F32>
 __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lanes_log) {
   typedef typename Elem<DT>::type T;
   typedef typename Elem<OUT_F32 ? CG_F32 : DT>::type O;
-  constexpr int V = Chunk<T>::V;
+  constexpr int V = Chunk<T, true>::V;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
   const int team = threadIdx.x >> lanes_log;
   if (blockIdx.x < a.chunk_groups) {  // parts of hot rows
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
       if (to - from <= a.span || (part == 1 && first == last)) continue;
       float *dst = a.partial + ((int64_t)chunk * 2 + part) * a.d;
       for (int32_t j = lane * V; j < a.d; j += lanes * V) {
-        Chunk<T> c;
+        Chunk<T, true> c;
         c.place(j, a.d);
         float sum[V];
         add_rows<T>(a, c, from > begin ? from : begin, to < end ? to : end, sum);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
     if (to - from > a.span || (from == to && a.beta == 1.f)) continue;
     O *out = (O *)a.out + v * a.ldo;
     for (int32_t j = lane * V; j < a.d; j += lanes * V) {
-      Chunk<T> c;
+      Chunk<T, true> c;
       c.place(j, a.d);
       float sum[V];
       add_rows<T>(a, c, from, to, sum);
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
   __shared__ float lds[kFoldWaves][kFoldColumns];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int32_t j = blockIdx.y * kFoldColumns + lane * 4, all = a.rowptr[a.rows];
-  Chunk<float> c;
+  Chunk<float, true> c;
   c.place(j, a.d);
   for (int32_t chunk = blockIdx.x; chunk < (int32_t)a.chunk_teams; chunk += gridDim.x) {  // uniform in the workgroup
     const int32_t begin = chunk * a.span;

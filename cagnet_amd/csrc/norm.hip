@@ -13,7 +13,7 @@ namespace cg {
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  __shared__ float slots[2][kNormWaves];
+  __shared__ NormSlots slots;
   int turn = 0;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
@@ -21,7 +21,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
     const T *z = (const T *)a.z + row * a.ldz;
     float s = 0.f;
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) s += (float)z[j] * (float)z[j];
-    const float rho_z = 1.f / sqrtf(row_sum<kNormThreads>(s, slots, turn) / (float)a.d + a.eps);
+    const float rho_z = 1.f / sqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_z[row] = rho_z;
     if (!RESIDUAL) {
       T *h = (T *)a.h + row * a.ldh;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
       r[j] = rounded<T>(v);
       s += v * v;
     }
-    const float rho_r = 1.f / sqrtf(row_sum<kNormThreads>(s, slots, turn) / (float)a.d + a.eps);
+    const float rho_r = 1.f / sqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_r[row] = rho_r;
     // h comes from the sum before its rounding to the stored type
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = rounded<T>(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a)
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  __shared__ float slots[2][kNormWaves];
+  __shared__ NormSlots slots;
   int turn = 0;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       float s = 0.f;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
         s += (float)dh[j] * weight_at<T>(a.w_post, a.w_f32, j) * ((float)z[j] * rho_z);
-      const float m = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
+      const float m = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
         const float zh = (float)z[j] * rho_z, g = (float)dh[j];
         q[j] += g * zh;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       float s = 0.f;
       for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
         s += (float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) * ((float)r[j] * rho_r);
-      mean_r = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
+      mean_r = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
     }
     auto into = [&](int32_t j) {  // gradient of the residual sum
       float v = dr ? (float)dr[j] : 0.f;
@@ -116,9 +116,9 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a)
       else if (dgate)
         dgate[j] = rounded<T>(dg);
     }
-    const float mean_z = row_sum<kNormThreads>(s, slots, turn) / (float)a.d;
+    const float mean_z = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
     if (a.gate_kind == CG_GATE_ROW) {
-      sg = row_sum<kNormThreads>(sg, slots, turn);
+      sg = row_sum<kWave, true>(sg, slots, turn);
       if (dgate && threadIdx.x == 0) dgate[0] = rounded<T>(sg);
     }
     for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
@@ -166,11 +166,12 @@ __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kerne
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-// Workgroups of a gradient = slices of partial sums: four per compute unit, two where a workgroup holds one row at a
-// time (long rows: the slices are as long and the loads of two workgroups keep the memory busy).
+// Workgroups of a gradient = slices of partial sums: enough for 16 wavefronts per compute unit, 12 where a workgroup
+// holds one row at a time (its slices are as long as its rows).
 static int64_t norm_groups(int64_t n, int32_t d, int dtype) {
   const NormShape sh = norm_shape(d, dtype);
-  const int64_t most = sh.lanes == 0 || sh.lanes == kNormThreads ? 512 : 1024;
+  const int waves = sh.threads / kWave, per_cu = (sh.whole ? 12 : 16) / waves;
+  const int64_t most = 256 * (per_cu > 0 ? per_cu : 1);
   const int64_t want = ceil_div64(n, norm_rows_at_once(sh));
   return want < most ? want : most;
 }

@@ -7,16 +7,16 @@
 namespace cg {
 
 // the workgroup's columns of one sum, added over its teams in a fixed order, to dst[0..d)
-template <typename T, int LANES, int K>
-__device__ __forceinline__ void fold_columns(float (&acc)[K][Chunk<T>::V], const Chunk<T> (&c)[K], float *lds,
-                                             float *__restrict__ dst, int32_t d) {
-  constexpr int V = Chunk<T>::V;
-  if (LANES > kWave) {  // every column belongs to one lane
+template <typename C, int LANES, int K, bool WHOLE>
+__device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)[K], float *lds, float *__restrict__ dst,
+                                             int32_t d) {
+  constexpr int V = C::V;
+  if (WHOLE) {  // every column belongs to one lane
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i < c[k].live) dst[((int)threadIdx.x + k * LANES) * V + i] = acc[k][i];
+        if (i < c[k].live) dst[((int)threadIdx.x + k * (int)blockDim.x) * V + i] = acc[k][i];
     return;
   }
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -38,26 +38,27 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][Chunk<T>::V], const
   __syncthreads();
 }
 
-template <int DT, int LANES, int K, bool RESIDUAL>
-__global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
+template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void norm_bwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T> C;
-  constexpr int V = C::V, TEAMS = kNormThreads / LANES;
-  __shared__ float slots[2][kNormWaves];
-  __shared__ float lds[LANES > kWave ? 1 : kNormWaves * LANES * K * V];
+  typedef Chunk<T, RAGGED> C;
+  constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
+  __shared__ NormSlots slots;
+  __shared__ float lds[WHOLE ? 1 : kNormWaves * LANES * K * V];
   int turn = 0;
-  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  const int lane = WHOLE ? threadIdx.x : threadIdx.x % LANES, team = WHOLE ? 0 : threadIdx.x / LANES;
+  const int lanes = WHOLE ? blockDim.x : LANES;
   C c[K];
   float wz[K][V], wr[K][V], q[K][V], p[K][V];  // alpha scale w_post (w_post alone for rms_norm), w_pre, column sums
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int32_t j = (lane + k * LANES) * V;
+    const int32_t j = (lane + k * lanes) * V;
     c[k].place(j, a.d);
-    weight_chunk<T>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
+    weight_chunk<T, V>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
     if (RESIDUAL) {
       float s[V];
-      weight_chunk<T>(a.scale, a.w_f32, j, c[k].live, s);
-      weight_chunk<T>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
+      weight_chunk<T, V>(a.scale, a.w_f32, j, c[k].live, s);
+      weight_chunk<T, V>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) wz[k][i] *= a.alpha * s[i];
     }
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
           s += t[k][i] * zh[k][i];
         }
       }
-      const float m = row_sum<LANES>(s, slots, turn) * inv_d;
+      const float m = row_sum<LANES, WHOLE>(s, slots, turn) * inv_d;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -131,7 +132,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
           s += D[k][i] * rh[k][i];
         }
       }
-      const float m = row_sum<LANES>(s, slots, turn) * inv_d;
+      const float m = row_sum<LANES, WHOLE>(s, slots, turn) * inv_d;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -157,12 +158,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
     for (int k = 0; k < K; ++k) {
       c[k].write((T *)a.dx + row * a.lddx, D[k]);
       c[k].floats(rz[k], zh[k]);
-      if (a.mask.rng) {
-        float m[V];
-        mask_chunk<V>(key, a.mask, row, (lane + k * LANES) * V, m);
-#pragma unroll
-        for (int i = 0; i < V; ++i) D[k][i] = m[i] > 0.f ? D[k][i] * m[i] : 0.f;
-      }
+      if (a.mask.rng)
+        drop_chunk<V>(key, a.mask, row, (lane + k * lanes) * V, D[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) zh[k][i] *= rho_z;
       if (a.gate_kind == CG_GATE_FULL) {
@@ -186,7 +183,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) s += D[k][i] * zh[k][i];
     }
-    s = row_sum<LANES>(s, slots, turn);
+    s = row_sum<LANES, WHOLE>(s, slots, turn);
     if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));
     const float m = s * inv_d, rho_s = rho_z * row_sig;
 #pragma unroll
@@ -197,49 +194,45 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormArgs a) {
     }
   }
   float *slice = a.partial + (int64_t)blockIdx.x * (RESIDUAL ? 2 : 1) * a.d;
-  fold_columns<T, LANES, K>(q, c, lds, slice, a.d);
-  if (RESIDUAL) fold_columns<T, LANES, K>(p, c, lds, slice + a.d, a.d);
+  fold_columns<C, LANES, K, WHOLE>(q, c, lds, slice, a.d);
+  if (RESIDUAL) fold_columns<C, LANES, K, WHOLE>(p, c, lds, slice + a.d, a.d);
 }
 
-template <int DT, int LANES, int K>
-static int go(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
+template <int DT, int LANES, int K, bool WHOLE, bool RAGGED>
+static int go_ragged(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
   if (residual)
-    norm_bwd_kernel<DT, LANES, K, true><<<(unsigned)groups, kNormThreads, 0, s>>>(a);
+    norm_bwd_kernel<DT, LANES, K, WHOLE, RAGGED, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   else
-    norm_bwd_kernel<DT, LANES, K, false><<<(unsigned)groups, kNormThreads, 0, s>>>(a);
+    norm_bwd_kernel<DT, LANES, K, WHOLE, RAGGED, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   CG_LAUNCH_CHECK();
   return CG_OK;
 }
 
+template <int DT, int LANES, int K, bool WHOLE>
+static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
+  if (a.d % (DT == CG_F32 ? 4 : 8) == 0) return go_ragged<DT, LANES, K, WHOLE, false>(a, residual, sh, groups, s);
+  return go_ragged<DT, LANES, K, WHOLE, true>(a, residual, sh, groups, s);
+}
+
 template <int DT>
-static int go_shape(const NormArgs &a, bool residual, const NormShape &sh, int64_t n, hipStream_t s) {
-  constexpr bool F32 = DT == CG_F32;
-  switch (sh.lanes * 16 + sh.chunks) {
-    case 4 * 16 + 1: return go<DT, 4, 1>(a, residual, n, s);
-    case 8 * 16 + 1: return go<DT, 8, 1>(a, residual, n, s);
-    case 16 * 16 + 1: return go<DT, 16, 1>(a, residual, n, s);
-    case 32 * 16 + 1: return go<DT, 32, 1>(a, residual, n, s);
-    case 64 * 16 + 1: return go<DT, 64, 1>(a, residual, n, s);
-    case 64 * 16 + 2: return go<DT, 64, 2>(a, residual, n, s);
-    case 64 * 16 + 3: if (F32) return go<DT, 64, F32 ? 3 : 1>(a, residual, n, s); break;
-    case 64 * 16 + 4: if (F32) return go<DT, 64, F32 ? 4 : 1>(a, residual, n, s); break;
-    case 256 * 16 + 1: if (!F32) return go<DT, 256, 1>(a, residual, n, s); break;
-    case 256 * 16 + 2: return go<DT, 256, 2>(a, residual, n, s);
-    case 256 * 16 + 3: return go<DT, 256, 3>(a, residual, n, s);
-    case 256 * 16 + 4: return go<DT, 256, 4>(a, residual, n, s);
-    case 256 * 16 + 5: if (F32) return go<DT, 256, F32 ? 5 : 2>(a, residual, n, s); break;
-    case 256 * 16 + 6: if (F32) return go<DT, 256, F32 ? 6 : 2>(a, residual, n, s); break;
-    case 256 * 16 + 7: if (F32) return go<DT, 256, F32 ? 7 : 2>(a, residual, n, s); break;
-    case 256 * 16 + 8: if (F32) return go<DT, 256, F32 ? 8 : 2>(a, residual, n, s); break;
-  }
-  CG_FAIL(CG_ERR_UNSUPPORTED, "norm: no kernel for %d lanes of %d chunks", sh.lanes, sh.chunks);
+static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
+  constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
+  const NormShape sh = norm_shape(a.d, DT);
+  if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);
+  if (sh.lanes == 4) return go<DT, 4, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 8) return go<DT, 8, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 16) return go<DT, 16, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 32) return go<DT, 32, 1, false>(a, residual, sh, groups, s);
+  if (sh.chunks == 1) return go<DT, kWave, 1, false>(a, residual, sh, groups, s);
+  if (sh.chunks == 2) return go<DT, kWave, 2, false>(a, residual, sh, groups, s);
+  if (MOST > 2 && sh.chunks == 3) return go<DT, kWave, MOST - 1, false>(a, residual, sh, groups, s);
+  return go<DT, kWave, MOST, false>(a, residual, sh, groups, s);
 }
 
 int launch_norm_bwd(const NormArgs &a, bool residual, int dtype, int64_t groups, hipStream_t s) {
-  const NormShape sh = norm_shape(a.d, dtype);
-  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, sh, groups, s);
-  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, sh, groups, s);
-  return go_shape<CG_F16>(a, residual, sh, groups, s);
+  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, groups, s);
+  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, groups, s);
+  return go_shape<CG_F16>(a, residual, groups, s);
 }
 
 }  // namespace cg

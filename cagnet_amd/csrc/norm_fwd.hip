@@ -5,25 +5,26 @@
 
 namespace cg {
 
-template <int DT, int LANES, int K, bool RESIDUAL>
-__global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormArgs a) {
+template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void norm_fwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T> C;
-  constexpr int V = C::V, TEAMS = kNormThreads / LANES;
-  __shared__ float slots[2][kNormWaves];
+  typedef Chunk<T, RAGGED> C;
+  constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
+  __shared__ NormSlots slots;
   int turn = 0;
-  const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+  const int lane = WHOLE ? threadIdx.x : threadIdx.x % LANES, team = WHOLE ? 0 : threadIdx.x / LANES;
+  const int lanes = WHOLE ? blockDim.x : LANES;
   C c[K];
   float wz[K][V], wr[K][V];  // alpha scale w_post (w_post alone for rms_norm) and w_pre
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int32_t j = (lane + k * LANES) * V;
+    const int32_t j = (lane + k * lanes) * V;
     c[k].place(j, a.d);
-    weight_chunk<T>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
+    weight_chunk<T, V>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
     if (RESIDUAL) {
       float s[V];
-      weight_chunk<T>(a.scale, a.w_f32, j, c[k].live, s);
-      weight_chunk<T>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
+      weight_chunk<T, V>(a.scale, a.w_f32, j, c[k].live, s);
+      weight_chunk<T, V>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) wz[k][i] *= a.alpha * s[i];
     }
@@ -54,7 +55,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[k][i] * v[k][i];
     }
-    const float rho_z = rsqrtf(row_sum<LANES>(s, slots, turn) * inv_d + a.eps);
+    const float rho_z = rsqrtf(row_sum<LANES, WHOLE>(s, slots, turn) * inv_d + a.eps);
     if (lane == 0) a.rstd_z[row] = rho_z;
     if (!RESIDUAL) {
 #pragma unroll
@@ -78,12 +79,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[k][i] *= sigmoid(g[i]);
       }
-      if (a.mask.rng) {
-        float m[V];
-        mask_chunk<V>(key, a.mask, row, (lane + k * LANES) * V, m);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[k][i] = m[i] > 0.f ? v[k][i] * m[i] : 0.f;
-      }
+      if (a.mask.rng)
+        drop_chunk<V>(key, a.mask, row, (lane + k * lanes) * V, v[k]);
       c[k].floats(rx[k], x);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -92,7 +89,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormArgs a) {
       }
       c[k].write((T *)a.r + row * a.ldr, v[k]);
     }
-    const float rho_r = rsqrtf(row_sum<LANES>(s, slots, turn) * inv_d + a.eps);
+    const float rho_r = rsqrtf(row_sum<LANES, WHOLE>(s, slots, turn) * inv_d + a.eps);
     if (lane == 0) a.rstd_r[row] = rho_r;
 #pragma unroll
     for (int k = 0; k < K; ++k) {  // h comes from the sum before its rounding to the stored type
@@ -103,47 +100,43 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormArgs a) {
   }
 }
 
-template <int DT, int LANES, int K>
-static int go(const NormArgs &a, bool residual, hipStream_t s) {
-  const int64_t want = ceil_div64(a.n, kNormThreads / LANES);
-  const unsigned groups = (unsigned)(want < 256 * 8 ? want : 256 * 8);
+template <int DT, int LANES, int K, bool WHOLE, bool RAGGED>
+static int go_ragged(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
   if (residual)
-    norm_fwd_kernel<DT, LANES, K, true><<<groups, kNormThreads, 0, s>>>(a);
+    norm_fwd_kernel<DT, LANES, K, WHOLE, RAGGED, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   else
-    norm_fwd_kernel<DT, LANES, K, false><<<groups, kNormThreads, 0, s>>>(a);
+    norm_fwd_kernel<DT, LANES, K, WHOLE, RAGGED, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   CG_LAUNCH_CHECK();
   return CG_OK;
 }
 
+template <int DT, int LANES, int K, bool WHOLE>
+static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
+  if (a.d % (DT == CG_F32 ? 4 : 8) == 0) return go_ragged<DT, LANES, K, WHOLE, false>(a, residual, sh, groups, s);
+  return go_ragged<DT, LANES, K, WHOLE, true>(a, residual, sh, groups, s);
+}
+
 template <int DT>
-static int go_shape(const NormArgs &a, bool residual, const NormShape &sh, hipStream_t s) {
-  constexpr bool F32 = DT == CG_F32;
-  switch (sh.lanes * 16 + sh.chunks) {
-    case 4 * 16 + 1: return go<DT, 4, 1>(a, residual, s);
-    case 8 * 16 + 1: return go<DT, 8, 1>(a, residual, s);
-    case 16 * 16 + 1: return go<DT, 16, 1>(a, residual, s);
-    case 32 * 16 + 1: return go<DT, 32, 1>(a, residual, s);
-    case 64 * 16 + 1: return go<DT, 64, 1>(a, residual, s);
-    case 64 * 16 + 2: return go<DT, 64, 2>(a, residual, s);
-    case 64 * 16 + 3: if (F32) return go<DT, 64, F32 ? 3 : 1>(a, residual, s); break;
-    case 64 * 16 + 4: if (F32) return go<DT, 64, F32 ? 4 : 1>(a, residual, s); break;
-    case 256 * 16 + 1: if (!F32) return go<DT, 256, 1>(a, residual, s); break;
-    case 256 * 16 + 2: return go<DT, 256, 2>(a, residual, s);
-    case 256 * 16 + 3: return go<DT, 256, 3>(a, residual, s);
-    case 256 * 16 + 4: return go<DT, 256, 4>(a, residual, s);
-    case 256 * 16 + 5: if (F32) return go<DT, 256, F32 ? 5 : 2>(a, residual, s); break;
-    case 256 * 16 + 6: if (F32) return go<DT, 256, F32 ? 6 : 2>(a, residual, s); break;
-    case 256 * 16 + 7: if (F32) return go<DT, 256, F32 ? 7 : 2>(a, residual, s); break;
-    case 256 * 16 + 8: if (F32) return go<DT, 256, F32 ? 8 : 2>(a, residual, s); break;
-  }
-  CG_FAIL(CG_ERR_UNSUPPORTED, "norm: no kernel for %d lanes of %d chunks", sh.lanes, sh.chunks);
+static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
+  constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
+  const NormShape sh = norm_shape(a.d, DT);
+  const int64_t want = ceil_div64(a.n, norm_rows_at_once(sh)), most = sh.whole ? 256 * 16 / (sh.threads / kWave) : 256 * 8;
+  groups = want < most ? want : most;
+  if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);
+  if (sh.lanes == 4) return go<DT, 4, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 8) return go<DT, 8, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 16) return go<DT, 16, 1, false>(a, residual, sh, groups, s);
+  if (sh.lanes == 32) return go<DT, 32, 1, false>(a, residual, sh, groups, s);
+  if (sh.chunks == 1) return go<DT, kWave, 1, false>(a, residual, sh, groups, s);
+  if (sh.chunks == 2) return go<DT, kWave, 2, false>(a, residual, sh, groups, s);
+  if (MOST > 2 && sh.chunks == 3) return go<DT, kWave, MOST - 1, false>(a, residual, sh, groups, s);
+  return go<DT, kWave, MOST, false>(a, residual, sh, groups, s);
 }
 
 int launch_norm_fwd(const NormArgs &a, bool residual, int dtype, hipStream_t s) {
-  const NormShape sh = norm_shape(a.d, dtype);
-  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, sh, s);
-  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, sh, s);
-  return go_shape<CG_F16>(a, residual, sh, s);
+  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, 0, s);
+  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, 0, s);
+  return go_shape<CG_F16>(a, residual, 0, s);
 }
 
 }  // namespace cg

@@ -25,10 +25,14 @@ struct NormArgs {
 
 // Lanes that share a row and 16-byte chunks each of them holds.  Rows of up to 64 chunks are taken by the smallest
 // power of two of lanes (at least 4) that covers them with one chunk each, several rows per wavefront; longer rows by a
-// whole wavefront with up to 16 elements a lane; then by a workgroup of 256 lanes with up to 32 elements a lane.
-// lanes == 0: the row does not fit and is read again for every pass over it.
+// whole wavefront with up to 16 elements a lane; then by a workgroup of as many wavefronts as the row fills with 16
+// elements a lane, at most 8.  lanes == 0: the row does not fit and is read again for every pass over it.
+constexpr int kNormMaxWaves = 8;
+
 struct NormShape {
   int lanes, chunks;
+  int threads;  // of a workgroup
+  bool whole;   // the workgroup holds one row at a time
 };
 static inline NormShape norm_shape(int32_t d, int dtype) {
   const int v = dtype == CG_F32 ? 4 : 8;
@@ -36,15 +40,15 @@ static inline NormShape norm_shape(int32_t d, int dtype) {
   if (c <= kWave) {
     int lanes = 4;
     while (lanes < c) lanes *= 2;
-    return NormShape{lanes, 1};
+    return NormShape{lanes, 1, kNormThreads, false};
   }
-  if (c <= (int64_t)kWave * (16 / v)) return NormShape{kWave, (int)ceil_div64(c, kWave)};
-  if (c <= (int64_t)kNormThreads * (32 / v)) return NormShape{kNormThreads, (int)ceil_div64(c, kNormThreads)};
-  return NormShape{0, 0};
+  const int most = 16 / v;  // chunks of 16 elements a lane
+  if (c <= (int64_t)kWave * most) return NormShape{kWave, (int)ceil_div64(c, kWave), kNormThreads, false};
+  const int64_t waves = ceil_div64(c, (int64_t)kWave * most);
+  if (waves <= kNormMaxWaves) return NormShape{kWave, most, (int)waves * kWave, true};
+  return NormShape{0, 0, kNormThreads, true};
 }
-static inline int norm_rows_at_once(const NormShape &s) {
-  return s.lanes == 0 || s.lanes == kNormThreads ? 1 : kNormThreads / s.lanes;
-}
+static inline int norm_rows_at_once(const NormShape &s) { return s.whole ? 1 : s.threads / s.lanes; }
 
 int launch_norm_fwd(const NormArgs &a, bool residual, int dtype, hipStream_t s);
 int launch_norm_bwd(const NormArgs &a, bool residual, int dtype, int64_t groups, hipStream_t s);
@@ -52,40 +56,45 @@ int launch_norm_bwd(const NormArgs &a, bool residual, int dtype, int64_t groups,
 // Sum over the lanes of a row.  Teams inside a wavefront exchange registers; a whole workgroup goes through `slots`,
 // whose halves alternate from one reduction to the next, so that one barrier a reduction is enough: a half is written
 // again only after everybody has passed the barrier of the reduction in between, hence has read it.
-template <int LANES>
-__device__ __forceinline__ float row_sum(float v, float (*slots)[kNormWaves], int &turn) {
+typedef float NormSlots[2][kNormMaxWaves];
+
+template <int LANES, bool WHOLE>
+__device__ __forceinline__ float row_sum(float v, NormSlots &slots, int &turn) {
 #pragma unroll
-  for (int off = (LANES < kWave ? LANES : kWave) / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  if (LANES <= kWave) return v;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  for (int off = LANES / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if (!WHOLE) return v;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   if (lane == 0) slots[turn][wave] = v;
   __syncthreads();
   float s = 0.f;
-#pragma unroll
-  for (int w = 0; w < kNormWaves; ++w) s += slots[turn][w];
+  for (int w = 0; w < waves; ++w) s += slots[turn][w];
   turn ^= 1;
   return s;
 }
 
-// v_rcp_f32 and v_rsq_f32 are within one unit of the last place; exp's argument is exact
-__device__ __forceinline__ float sigmoid(float a) { return __builtin_amdgcn_rcpf(1.f + expf(-a)); }
-
-// a weight vector's elements of one chunk, ones for a null pointer, zeros behind the row's end
-template <typename T>
-__device__ __forceinline__ void weight_chunk(const void *w, int w_f32, int32_t j, int live, float (&out)[Chunk<T>::V]) {
-#pragma unroll
-  for (int i = 0; i < Chunk<T>::V; ++i) out[i] = i < live ? weight_at<T>(w, w_f32, j + i) : 0.f;
+// 1 / (1 + 2^(-a log2 e)).  The hardware's exponential and reciprocal are within one unit of the last place; the
+// rounding of the exponent adds |a| roundings to e^-a, which for a > 0 is the small term of the sum and for a < 0 leaves
+// a result below e^a off by |a| e^a units.
+__device__ __forceinline__ float sigmoid(float a) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504f));
 }
 
-// 1 / (1 - p) or 0 for the elements of the chunk that starts at column j (a multiple of four)
+// a weight vector's elements of one chunk, ones for a null pointer, zeros behind the row's end
+template <typename T, int V>
+__device__ __forceinline__ void weight_chunk(const void *w, int w_f32, int32_t j, int live, float (&out)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[i] = i < live ? weight_at<T>(w, w_f32, j + i) : 0.f;
+}
+
+// v / (1 - p) for the kept elements of the chunk that starts at column j (a multiple of four), 0 for the others
 template <int V>
-__device__ __forceinline__ void mask_chunk(const MaskKey &k, const Mask &m, int64_t row, int32_t j, float (&out)[V]) {
+__device__ __forceinline__ void drop_chunk(const MaskKey &k, const Mask &m, int64_t row, int32_t j, float (&v)[V]) {
 #pragma unroll
   for (int b = 0; b < V / 4; ++b) {
     uint32_t w[4];
     mask_words(k, (uint32_t)row, (uint32_t)(j / 4 + b), w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out[4 * b + i] = w[i] > m.last ? m.inv_keep : 0.f;
+    for (int i = 0; i < 4; ++i) v[4 * b + i] = w[i] > m.last ? v[4 * b + i] * m.inv_keep : 0.f;
   }
 }
 

@@ -72,19 +72,20 @@ __device__ __forceinline__ void store_some(T *__restrict__ p, int live, const fl
 }
 
 // ---------------------------------------------------------------------------------------------
-// A row as 16-byte chunks, one per lane and step.  Every load is unconditional: the last chunk of a row that does not
-// fill one reads the row's last 16 bytes and is shifted into place, lanes behind the row's end read its start and are
-// zeroed.  A load behind a branch would make the compiler wait for it inside the branch.
+// A row as 16-byte chunks, one per lane and step.  Every load is unconditional: a load behind a branch would make the
+// compiler wait for it inside the branch.  Lanes behind the row's end read its start and are zeroed.  RAGGED: rows whose
+// length is not a whole number of chunks; the last chunk is then read as the row's last 16 bytes and shifted into place,
+// which costs up to 20 instructions a load, so that rows of whole chunks have kernels of their own.
 // ---------------------------------------------------------------------------------------------
 typedef uint32_t Raw __attribute__((ext_vector_type(4)));
 
-template <typename T>
+template <typename T, bool RAGGED>
 struct Chunk {
   static constexpr int V = 16 / (int)sizeof(T);  // elements of a chunk
   typedef typename Pack<T, V>::type vec;
 
-  int32_t at;   // element of the row the load starts at
-  int32_t live; // elements of the row in this chunk: V, fewer in the last one, 0 behind the end
+  int32_t at;    // element of the row the load starts at
+  int32_t live;  // elements of the row in this chunk: V, fewer in the last one, 0 behind the end
   int32_t d;
 
   __device__ __forceinline__ void place(int32_t j, int32_t d_) {
@@ -94,7 +95,7 @@ struct Chunk {
     at = left >= V ? j : (left > 0 && d >= V ? d - V : 0);
   }
   __device__ __forceinline__ Raw load(const T *row) const {
-    if (d >= V) return __builtin_bit_cast(Raw, *reinterpret_cast<const vec *>(row + at));
+    if (!RAGGED || d >= V) return __builtin_bit_cast(Raw, *reinterpret_cast<const vec *>(row + at));
     vec q = {};  // rows shorter than a chunk (uniform branch)
 #pragma unroll
     for (int i = 0; i < V; ++i) q[i] = row[i < d ? i : d - 1];
@@ -102,36 +103,36 @@ struct Chunk {
   }
   // the chunk's elements as floats; those that are not live are zero
   __device__ __forceinline__ void floats(Raw r, float (&out)[V]) const {
-    if (d >= V && d % V != 0) {  // uniform: rows with a partial chunk
-      const int32_t drop = live > 0 ? V - live : 0;  // elements of the chunk before that this load repeats
+    if (!RAGGED) {
+      r = live ? r : Raw{0u, 0u, 0u, 0u};
+    } else if (d >= V) {  // uniform
+      const int32_t drop = V - live;  // elements of the chunk before that this load repeats; all V behind the end
       if (sizeof(T) == 4) {
         r = (drop & 1) ? Raw{r.y, r.z, r.w, 0u} : r;
         r = (drop & 2) ? Raw{r.z, r.w, 0u, 0u} : r;
+        r = (drop & 4) ? Raw{0u, 0u, 0u, 0u} : r;
       } else {
         r = (drop & 1) ? Raw{(r.x >> 16) | (r.y << 16), (r.y >> 16) | (r.z << 16), (r.z >> 16) | (r.w << 16), r.w >> 16} : r;
         r = (drop & 2) ? Raw{r.y, r.z, r.w, 0u} : r;
         r = (drop & 4) ? Raw{r.z, r.w, 0u, 0u} : r;
+        r = (drop & 8) ? Raw{0u, 0u, 0u, 0u} : r;
       }
     }
     const vec q = __builtin_bit_cast(vec, r);
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = (float)q[i];
-    if (d < V) {
+    if (RAGGED && d < V) {
 #pragma unroll
       for (int i = 0; i < V; ++i) out[i] = i < live ? out[i] : 0.f;
-    } else if (live == 0) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) out[i] = 0.f;
     }
   }
-  __device__ __forceinline__ void read(const T *row, float (&out)[V]) const { floats(load(row), out); }
   __device__ __forceinline__ void write(T *row, const float (&in)[V]) const {
     vec q = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) q[i] = rounded<T>(in[i]);
     if (live == V) {
       *reinterpret_cast<vec *>(row + at) = q;
-    } else if (live > 0) {
+    } else if (RAGGED && live > 0) {
       T *p = row + d - live;
 #pragma unroll
       for (int i = 0; i < V - 1; ++i)
