@@ -168,8 +168,8 @@ __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kerne
 // ---- host side ------------------------------------------------------------------------------------
 // Workgroups of a gradient = slices of partial sums: enough for 16 wavefronts per compute unit, 12 where a workgroup
 // holds one row at a time (its slices are as long as its rows).
-static int64_t norm_groups(int64_t n, int32_t d, int dtype) {
-  const NormShape sh = norm_shape(d, dtype);
+static int64_t norm_groups(int64_t n, int32_t d, int dtype, bool residual) {
+  const NormShape sh = norm_shape(d, dtype, residual);
   const int waves = sh.threads / kWave, per_cu = (sh.whole ? 12 : 16) / waves;
   const int64_t most = 256 * (per_cu > 0 ? per_cu : 1);
   const int64_t want = ceil_div64(n, norm_rows_at_once(sh));
@@ -177,12 +177,13 @@ static int64_t norm_groups(int64_t n, int32_t d, int dtype) {
 }
 // an upper bound for every type and both operators
 static size_t norm_workspace(int64_t n, int32_t d) {
-  int64_t groups = 0;
-  for (int dtype : {CG_F32, CG_BF16}) {
-    const int64_t g = norm_groups(n, d, dtype);
-    groups = g > groups ? g : groups;
-  }
-  return (size_t)groups * 2 * (size_t)d * sizeof(float);
+  int64_t slices = 0;  // of d floats
+  for (int dtype : {CG_F32, CG_BF16})
+    for (int residual : {0, 1}) {
+      const int64_t g = norm_groups(n, d, dtype, residual) * (residual ? 2 : 1);
+      slices = g > slices ? g : slices;
+    }
+  return (size_t)slices * (size_t)d * sizeof(float);
 }
 
 static int check_weights(const char *who, int dtype, int wdtype) {
@@ -198,7 +199,7 @@ static int check_float(const char *who, const char *what, float v, bool positive
 
 template <bool RESIDUAL>
 static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
-  if (norm_shape(a.d, dtype).lanes > 0) return launch_norm_fwd(a, RESIDUAL, dtype, s);
+  if (norm_shape(a.d, dtype, false).lanes > 0) return launch_norm_fwd(a, RESIDUAL, dtype, s);
   const int64_t groups = a.n < 256 * 32 ? a.n : 256 * 32;
 #define CG_CALL(DT) norm_fwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
   CG_BY_DTYPE(dtype, CG_CALL)
@@ -209,8 +210,8 @@ static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
 
 template <bool RESIDUAL>
 static int norm_bwd(const NormArgs &a, int dtype, void *dw_post, void *dw_pre, void *dscale, hipStream_t s) {
-  const int64_t groups = norm_groups(a.n, a.d, dtype);
-  if (groups > 0 && norm_shape(a.d, dtype).lanes > 0) {
+  const int64_t groups = norm_groups(a.n, a.d, dtype, RESIDUAL);
+  if (groups > 0 && norm_shape(a.d, dtype, RESIDUAL).lanes > 0) {
     CG_TRY(launch_norm_bwd(a, RESIDUAL, dtype, groups, s));
   } else if (groups > 0) {
 #define CG_CALL(DT) norm_bwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)

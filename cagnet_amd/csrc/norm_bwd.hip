@@ -217,7 +217,8 @@ static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t gro
 template <int DT>
 static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
   constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
-  const NormShape sh = norm_shape(a.d, DT);
+  const NormShape sh = norm_shape(a.d, DT, residual);
+  if (sh.whole && sh.chunks < MOST) return go<DT, kWave, MOST / 2, true>(a, residual, sh, groups, s);
   if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);
   if (sh.lanes == 4) return go<DT, 4, 1, false>(a, residual, sh, groups, s);
   if (sh.lanes == 8) return go<DT, 8, 1, false>(a, residual, sh, groups, s);

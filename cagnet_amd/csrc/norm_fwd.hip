@@ -119,7 +119,7 @@ static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t gro
 template <int DT>
 static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
   constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
-  const NormShape sh = norm_shape(a.d, DT);
+  const NormShape sh = norm_shape(a.d, DT, false);
   const int64_t want = ceil_div64(a.n, norm_rows_at_once(sh)), most = sh.whole ? 256 * 16 / (sh.threads / kWave) : 256 * 8;
   groups = want < most ? want : most;
   if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);

@@ -25,8 +25,10 @@ struct NormArgs {
 
 // Lanes that share a row and 16-byte chunks each of them holds.  Rows of up to 64 chunks are taken by the smallest
 // power of two of lanes (at least 4) that covers them with one chunk each, several rows per wavefront; longer rows by a
-// whole wavefront with up to 16 elements a lane; then by a workgroup of as many wavefronts as the row fills with 16
-// elements a lane, at most 8.  lanes == 0: the row does not fit and is read again for every pass over it.
+// whole wavefront with up to 16 elements a lane; then by a workgroup of as many wavefronts as the row fills, at most 8,
+// with 16 elements a lane.  The gradient of the residual block keeps five operands of a row and four column vectors in
+// registers: 8 elements a lane let three or four wavefronts run on a SIMD instead of two, and it takes 16 only where 8
+// wavefronts of 8 are too few.  lanes == 0: the row does not fit and is read again for every pass over it.
 constexpr int kNormMaxWaves = 8;
 
 struct NormShape {
@@ -34,7 +36,7 @@ struct NormShape {
   int threads;  // of a workgroup
   bool whole;   // the workgroup holds one row at a time
 };
-static inline NormShape norm_shape(int32_t d, int dtype) {
+static inline NormShape norm_shape(int32_t d, int dtype, bool residual_bwd) {
   const int v = dtype == CG_F32 ? 4 : 8;
   const int64_t c = ceil_div64(d, v);
   if (c <= kWave) {
@@ -44,8 +46,10 @@ static inline NormShape norm_shape(int32_t d, int dtype) {
   }
   const int most = 16 / v;  // chunks of 16 elements a lane
   if (c <= (int64_t)kWave * most) return NormShape{kWave, (int)ceil_div64(c, kWave), kNormThreads, false};
-  const int64_t waves = ceil_div64(c, (int64_t)kWave * most);
-  if (waves <= kNormMaxWaves) return NormShape{kWave, most, (int)waves * kWave, true};
+  for (int chunks = residual_bwd ? most / 2 : most; chunks <= most; chunks *= 2) {
+    const int64_t waves = ceil_div64(c, (int64_t)kWave * chunks);
+    if (waves <= kNormMaxWaves) return NormShape{kWave, chunks, (int)waves * kWave, true};
+  }
   return NormShape{0, 0, kNormThreads, true};
 }
 static inline int norm_rows_at_once(const NormShape &s) { return s.whole ? 1 : s.threads / s.lanes; }
