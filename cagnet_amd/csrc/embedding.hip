@@ -71,8 +71,8 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typena
 // ---------------------------------------------------------------------------------------------
 constexpr int kMaxDigit = 9;
 constexpr int kMaxRadix = 1 << kMaxDigit;
-constexpr int kKeysPerLane = 8;
-constexpr int kEmbTile = kEmbThreads * kKeysPerLane;  // 2048 keys a workgroup
+constexpr int kKeysPerLane = 4;
+constexpr int kEmbTile = kEmbThreads * kKeysPerLane;  // 1024 keys a workgroup
 constexpr int kWaveKeys = kWave * kKeysPerLane;
 
 // Where a pass reads its keys from: the caller's indices (an index outside the table becomes `rows`, which sorts
@@ -148,7 +148,7 @@ __device__ __forceinline__ uint32_t group_exclusive(uint32_t v, uint32_t *wave_s
   return before + inc - v;
 }
 
-// Wave w of a workgroup owns keys [tile + 512 w, tile + 512 (w + 1)), 64 at a time in order.  Lanes with equal digits
+// Wave w of a workgroup owns keys [tile + 256 w, tile + 256 (w + 1)), 64 at a time in order.  Lanes with equal digits
 // find each other by ballots; a key's rank is the wave's running count of its digit plus the equal lanes below it.
 __global__ __launch_bounds__(kEmbThreads) void emb_scatter_kernel(KeySource src, int64_t n, int shift, int dbits,
                                                                   const uint32_t *__restrict__ hist, int64_t tiles,
@@ -255,27 +255,37 @@ struct SumArgs {
   unsigned chunk_groups, chunk_teams;
 };
 
-constexpr int kAhead = 4;  // rows of g in flight per lane
+constexpr int kAhead = 8;  // rows of g in flight per lane
 
-// the chunk's columns of g's rows pos[from .. to), added in order
+// The chunk's columns of g's rows pos[from .. to), added in order.  The positions of the next kAhead rows are loaded
+// while those before them are on their way, so that a long segment pays one memory latency a step and not two.
 template <typename T>
 __device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T, true> &c, int32_t from, int32_t to,
                                          float (&sum)[Chunk<T, true>::V]) {
+  constexpr int V = Chunk<T, true>::V;
 #pragma unroll
-  for (int i = 0; i < Chunk<T, true>::V; ++i) sum[i] = 0.f;
+  for (int i = 0; i < V; ++i) sum[i] = 0.f;
+  if (from >= to) return;
+  int32_t p[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) p[k] = a.pos[from + k < to ? from + k : to - 1];
   for (int32_t at = from; at < to; at += kAhead) {
-    int32_t p[kAhead];
     Raw r[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) p[k] = a.pos[at + k < to ? at + k : to - 1];
+    for (int k = 0; k < kAhead; ++k) {
+      r[k] = Raw{0u, 0u, 0u, 0u};
+      if (k == 0 || at + k < to) r[k] = c.load((const T *)a.g + (int64_t)p[k] * a.ldg);
+    }
+    if (at + kAhead < to) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) r[k] = c.load((const T *)a.g + (int64_t)p[k] * a.ldg);
+      for (int k = 0; k < kAhead; ++k) p[k] = a.pos[at + kAhead + k < to ? at + kAhead + k : to - 1];
+    }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      float f[Chunk<T, true>::V];
+      float f[V];
       c.floats(r[k], f);
 #pragma unroll
-      for (int i = 0; i < Chunk<T, true>::V; ++i) sum[i] += at + k < to ? f[i] : 0.f;
+      for (int i = 0; i < V; ++i) sum[i] += f[i];
     }
   }
 }
@@ -353,7 +363,7 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
     const int32_t chunks = (to - 1) / a.span - chunk + 1;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     if (c.live > 0) {
-#pragma unroll 4
+#pragma unroll 8
       for (int32_t k = wave; k < chunks; k += kFoldWaves) {
         // the row's part in its first chunk is that chunk's last part unless the chunk begins with it
         const int64_t slot = (int64_t)(chunk + k) * 2 + (k == 0 && from > begin ? 1 : 0);
@@ -398,9 +408,9 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.passes = bits > 0 ? (bits + kMaxDigit - 1) / kMaxDigit : 1;
   p.dbits = bits > 0 ? (bits + p.passes - 1) / p.passes : 1;
   p.tiles = ceil_div64(n, kEmbTile);
-  // about sqrt(n) / 4: the longest chain of additions in a team and the longest list of partial rows grow alike
+  // about sqrt(n / 128): the longest chain of additions in a team and the longest list of partial rows grow alike
   p.span = 32;
-  while (p.span < 512 && (int64_t)p.span * p.span * 16 < n) p.span *= 2;
+  while (p.span < 512 && (int64_t)p.span * p.span * 128 < n) p.span *= 2;
   p.chunks = ceil_div64(n, p.span);
   size_t at = 0;
   auto take = [&at](size_t bytes) {

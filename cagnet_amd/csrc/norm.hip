@@ -166,11 +166,11 @@ __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kerne
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-// Workgroups of a gradient = slices of partial sums: enough for 16 wavefronts per compute unit, 12 where a workgroup
-// holds one row at a time (its slices are as long as its rows).
+// Workgroups of a gradient = slices of partial sums: enough for 16 wavefronts per compute unit; where a workgroup
+// holds one row at a time (its slices are as long as its rows) for 12 of the residual block's and 8 of rms_norm's.
 static int64_t norm_groups(int64_t n, int32_t d, int dtype, bool residual) {
   const NormShape sh = norm_shape(d, dtype, residual);
-  const int waves = sh.threads / kWave, per_cu = (sh.whole ? 12 : 16) / waves;
+  const int waves = sh.threads / kWave, per_cu = (!sh.whole ? 16 : residual ? 12 : 8) / waves;
   const int64_t most = 256 * (per_cu > 0 ? per_cu : 1);
   const int64_t want = ceil_div64(n, norm_rows_at_once(sh));
   return want < most ? want : most;
