@@ -67,13 +67,17 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typena
 }
 
 // ---------------------------------------------------------------------------------------------
-// stable radix sort of (key, position), digits of up to 9 bits: 16 to 18 bit tables take two passes
+// Stable radix sort of (key, position), digits of up to 9 bits: tables of 2^16 to 2^18 rows take two passes.  A
+// workgroup of 16 wavefronts holds a tile of 4096 keys.  One tile is sorted in LDS by one launch; up to kDirectTiles
+// tiles take two launches a pass (count, scatter: every scatter workgroup adds the tiles' counts up itself, one row of
+// counts a tile); more tiles take a third that scans the counts, one wavefront a digit.
 // ---------------------------------------------------------------------------------------------
-constexpr int kMaxDigit = 9;
-constexpr int kMaxRadix = 1 << kMaxDigit;
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
+constexpr int kMaxDigit = 9, kMaxRadix = 1 << kMaxDigit;
 constexpr int kKeysPerLane = 4;
-constexpr int kEmbTile = kEmbThreads * kKeysPerLane;  // 1024 keys a workgroup
+constexpr int kSortTile = kSortThreads * kKeysPerLane;
 constexpr int kWaveKeys = kWave * kKeysPerLane;
+constexpr int kDirectTiles = 64;
 
 // Where a pass reads its keys from: the caller's indices (an index outside the table becomes `rows`, which sorts
 // behind every table row) or the arrays of the pass before.
@@ -88,28 +92,29 @@ __device__ __forceinline__ int32_t key_at(const KeySource &s, int64_t i) {
   return (int32_t)(v >= 0 && v < s.rows ? v : s.rows);
 }
 
-// hist[digit * tiles + tile]
-__global__ __launch_bounds__(kEmbThreads) void emb_hist_kernel(KeySource src, int64_t n, int shift, int dbits,
-                                                               uint32_t *__restrict__ hist, int64_t tiles) {
+// Counts of a tile's digits, at hist[digit * digit_step + tile * tile_step].
+__global__ __launch_bounds__(kSortThreads) void emb_hist_kernel(KeySource src, int64_t n, int shift, int dbits,
+                                                                uint32_t *__restrict__ hist, int64_t digit_step,
+                                                                int64_t tile_step) {
   __shared__ uint32_t count[kMaxRadix];
   const int radix = 1 << dbits;
-  for (int i = threadIdx.x; i < radix; i += kEmbThreads) count[i] = 0;
-  __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kEmbTile;
+  if ((int)threadIdx.x < radix) count[threadIdx.x] = 0;
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
   int32_t k[kKeysPerLane];
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r) {
-    const int64_t i = base + r * kEmbThreads + threadIdx.x;
+    const int64_t i = base + r * kSortThreads + threadIdx.x;
     k[r] = key_at(src, i < n ? i : n - 1);
   }
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r)
-    if (base + r * kEmbThreads + threadIdx.x < n) atomicAdd(&count[((uint32_t)k[r] >> shift) & (radix - 1)], 1u);
+    if (base + r * kSortThreads + threadIdx.x < n) atomicAdd(&count[((uint32_t)k[r] >> shift) & (radix - 1)], 1u);
   __syncthreads();
-  for (int i = threadIdx.x; i < radix; i += kEmbThreads) hist[(int64_t)i * tiles + blockIdx.x] = count[i];
+  if ((int)threadIdx.x < radix) hist[threadIdx.x * digit_step + blockIdx.x * tile_step] = count[threadIdx.x];
 }
 
-// one wave per digit: exclusive prefix of its counts over the tiles, in place, and their total
+// one wavefront per digit: exclusive prefix of its counts over the tiles, in place, and their total
 __global__ __launch_bounds__(kEmbThreads) void emb_scan_kernel(uint32_t *__restrict__ hist, int64_t tiles, int radix,
                                                                uint32_t *__restrict__ totals) {
   const int digit = blockIdx.x * kEmbWaves + threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
@@ -131,6 +136,13 @@ __global__ __launch_bounds__(kEmbThreads) void emb_scan_kernel(uint32_t *__restr
   if (lane == 0) totals[digit] = run;
 }
 
+struct SortLds {
+  uint32_t count[kSortWaves][kMaxRadix];  // of a wavefront's digits, then their offsets in the tile
+  uint32_t before[kSortThreads], all[kSortThreads];
+  uint32_t wave_sums[kSortWaves];
+  int32_t key[kSortTile], pos[kSortTile];
+};
+
 // Exclusive prefix over the workgroup's threads of one value each.
 __device__ __forceinline__ uint32_t group_exclusive(uint32_t v, uint32_t *wave_sums) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -144,37 +156,24 @@ __device__ __forceinline__ uint32_t group_exclusive(uint32_t v, uint32_t *wave_s
   if (lane == kWave - 1) wave_sums[wave] = inc;
   __syncthreads();
   uint32_t before = 0;
-  for (int w = 0; w < wave; ++w) before += wave_sums[w];
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) before += w < wave ? wave_sums[w] : 0u;
   return before + inc - v;
 }
 
-// Wave w of a workgroup owns keys [tile + 256 w, tile + 256 (w + 1)), 64 at a time in order.  Lanes with equal digits
-// find each other by ballots; a key's rank is the wave's running count of its digit plus the equal lanes below it.
-__global__ __launch_bounds__(kEmbThreads) void emb_scatter_kernel(KeySource src, int64_t n, int shift, int dbits,
-                                                                  const uint32_t *__restrict__ hist, int64_t tiles,
-                                                                  const uint32_t *__restrict__ totals,
-                                                                  int32_t *__restrict__ out_key,
-                                                                  int32_t *__restrict__ out_pos) {
-  __shared__ uint32_t count[kEmbWaves][kMaxRadix];
-  __shared__ uint32_t first[kMaxRadix];  // global position of a record = first[digit] + its position in the tile
-  __shared__ uint32_t wave_sums[kEmbWaves];
-  __shared__ int32_t skey[kEmbTile], spos[kEmbTile];
+// Orders the tile's `here` keys by one digit in LDS; thread t < radix gets the first place of digit t in the tile.
+// Wave w owns keys [256 w, 256 (w + 1)) of the tile, 64 at a time in order.  Lanes with equal digits find each other
+// by ballots; a key's rank is the wave's running count of its digit plus the equal lanes below it.
+__device__ __forceinline__ uint32_t sort_tile(SortLds &s, const int32_t (&key)[kKeysPerLane], const int32_t (&pos)[kKeysPerLane],
+                                              int here, int shift, int dbits) {
   const int radix = 1 << dbits, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  for (int i = threadIdx.x; i < kEmbWaves * kMaxRadix; i += kEmbThreads) (&count[0][0])[i] = 0;
-  const int64_t tile_base = (int64_t)blockIdx.x * kEmbTile, base = tile_base + wave * kWaveKeys;
-  int32_t key[kKeysPerLane], pos[kKeysPerLane];
-#pragma unroll
-  for (int r = 0; r < kKeysPerLane; ++r) {
-    const int64_t i = base + r * kWave + lane, at = i < n ? i : n - 1;
-    key[r] = key_at(src, at);
-    pos[r] = src.pos ? src.pos[at] : (int32_t)at;
-  }
+  for (int i = threadIdx.x; i < kSortWaves * radix; i += kSortThreads) s.count[i >> dbits][i & (radix - 1)] = 0;
   __syncthreads();
   uint32_t rank[kKeysPerLane];
   const uint64_t below = (1ull << lane) - 1ull;
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r) {
-    const bool valid = base + r * kWave + lane < n;
+    const bool valid = wave * kWaveKeys + r * kWave + lane < here;
     const uint32_t digit = ((uint32_t)key[r] >> shift) & (uint32_t)(radix - 1);
     uint64_t peers = __ballot(valid);
 #pragma unroll
@@ -184,91 +183,155 @@ __global__ __launch_bounds__(kEmbThreads) void emb_scatter_kernel(KeySource src,
         const uint64_t with = __ballot(one);
         peers &= one ? with : ~with;
       }
-    const uint32_t before = (uint32_t)__popcll(peers & below);
+    const uint32_t lower = (uint32_t)__popcll(peers & below);
     uint32_t had = 0;
-    if (valid) had = count[wave][digit];
+    if (valid) had = s.count[wave][digit];
     // the lowest lane of the set writes the new count; it depends on `had`, so the read above comes first
-    if (valid && before == 0) count[wave][digit] = had + (uint32_t)__popcll(peers);
-    rank[r] = had + before;
+    if (valid && lower == 0) s.count[wave][digit] = had + (uint32_t)__popcll(peers);
+    rank[r] = had + lower;
   }
   __syncthreads();
-  // digit offsets: two digits a thread; in the tile (for the order in LDS) and in the whole array
-  const int d0 = threadIdx.x * 2;
-  uint32_t here[2] = {0, 0}, all[2] = {0, 0};
+  uint32_t mine = 0;
+  if ((int)threadIdx.x < radix)
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (d0 + k < radix) {
-      for (int w = 0; w < kEmbWaves; ++w) here[k] += count[w][d0 + k];
-      all[k] = totals[d0 + k];
-    }
-  uint32_t in_tile = group_exclusive(here[0] + here[1], wave_sums);
-  uint32_t in_all = group_exclusive(all[0] + all[1], wave_sums);
+    for (int w = 0; w < kSortWaves; ++w) mine += s.count[w][threadIdx.x];
+  const uint32_t first = group_exclusive(mine, s.wave_sums);
+  if ((int)threadIdx.x < radix) {
+    uint32_t run = first;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (d0 + k < radix) {
-      first[d0 + k] = in_all + hist[(int64_t)(d0 + k) * tiles + blockIdx.x] - in_tile;  // modulo 2^32, undone below
-      uint32_t run = in_tile;
-      for (int w = 0; w < kEmbWaves; ++w) {
-        const uint32_t c = count[w][d0 + k];
-        count[w][d0 + k] = run;
-        run += c;
-      }
-      in_tile += here[k];
-      in_all += all[k];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = s.count[w][threadIdx.x];
+      s.count[w][threadIdx.x] = run;
+      run += c;
     }
+  }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r)
-    if (base + r * kWave + lane < n) {
+    if (wave * kWaveKeys + r * kWave + lane < here) {
       const uint32_t digit = ((uint32_t)key[r] >> shift) & (uint32_t)(radix - 1);
-      const uint32_t at = count[wave][digit] + rank[r];
-      skey[at] = key[r];
-      spos[at] = pos[r];
+      const uint32_t at = s.count[wave][digit] + rank[r];
+      s.key[at] = key[r];
+      s.pos[at] = pos[r];
     }
   __syncthreads();
-  const int64_t left = n - tile_base;
-  const int here_n = (int)(left < kEmbTile ? left : kEmbTile);
-  for (int i = threadIdx.x; i < here_n; i += kEmbThreads) {
-    const uint32_t to = first[((uint32_t)skey[i] >> shift) & (uint32_t)(radix - 1)] + (uint32_t)i;
-    out_key[to] = skey[i];
-    out_pos[to] = spos[i];
+  return first;
+}
+
+// DIRECT: hist holds one row of counts per tile; otherwise the scanned counts of emb_scan_kernel, one row per digit.
+template <bool DIRECT>
+__global__ __launch_bounds__(kSortThreads) void emb_scatter_kernel(KeySource src, int64_t n, int shift, int dbits,
+                                                                   const uint32_t *__restrict__ hist, int64_t tiles,
+                                                                   const uint32_t *__restrict__ totals,
+                                                                   int32_t *__restrict__ out_key,
+                                                                   int32_t *__restrict__ out_pos, int32_t *hot_count) {
+  __shared__ SortLds s;
+  const int radix = 1 << dbits, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int64_t tile_base = (int64_t)blockIdx.x * kSortTile, left = n - tile_base;
+  const int here = (int)(left < kSortTile ? left : kSortTile);
+  if (hot_count && blockIdx.x == 0 && threadIdx.x == 0) *hot_count = 0;
+  int32_t key[kKeysPerLane], pos[kKeysPerLane];
+#pragma unroll
+  for (int r = 0; r < kKeysPerLane; ++r) {
+    const int64_t i = tile_base + wave * kWaveKeys + r * kWave + lane, at = i < n ? i : n - 1;
+    key[r] = key_at(src, at);
+    pos[r] = src.pos ? src.pos[at] : (int32_t)at;
+  }
+  uint32_t before = 0, all = 0;  // of digit threadIdx.x % radix: in the tiles below, in all of them
+  if (DIRECT) {
+    const int digit = threadIdx.x & (radix - 1), parts = kSortThreads >> dbits;
+#pragma unroll 8
+    for (int t = threadIdx.x >> dbits; t < (int)tiles; t += parts) {
+      const uint32_t c = hist[(int64_t)t * radix + digit];
+      before += t < (int)blockIdx.x ? c : 0u;
+      all += c;
+    }
+    s.before[threadIdx.x] = before;
+    s.all[threadIdx.x] = all;
+    __syncthreads();
+    before = all = 0;
+    if ((int)threadIdx.x < radix)
+      for (int k = 0; k < parts; ++k) {
+        before += s.before[(k << dbits) + threadIdx.x];
+        all += s.all[(k << dbits) + threadIdx.x];
+      }
+  } else if ((int)threadIdx.x < radix) {
+    before = hist[(int64_t)threadIdx.x * tiles + blockIdx.x];
+    all = totals[threadIdx.x];
+  }
+  const uint32_t start = group_exclusive(all, s.wave_sums);
+  const uint32_t first = sort_tile(s, key, pos, here, shift, dbits);
+  // global place of a record = first place of its digit here + its place in the tile, modulo 2^32
+  if ((int)threadIdx.x < radix) s.before[threadIdx.x] = start + before - first;
+  __syncthreads();
+  for (int i = threadIdx.x; i < here; i += kSortThreads) {
+    const uint32_t to = s.before[((uint32_t)s.key[i] >> shift) & (uint32_t)(radix - 1)] + (uint32_t)i;
+    out_key[to] = s.key[i];
+    out_pos[to] = s.pos[i];
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Sums.  rowptr[v] .. rowptr[v + 1] are the sorted positions of table row v.  A row with up to `span` of them is added
-// up by one team of lanes.  The sorted array is also cut into chunks of `span` positions: a row with more than `span`
-// ("hot": with popular indices one row can hold a tenth of all) covers the end of at least one chunk, so a chunk holds a
-// part of at most two hot rows, the one it begins in and the one it ends in.  A team adds up each part into a partial
-// row, and a second kernel adds a hot row's partial rows in order.
+// Sums.  The sorted array is cut into chunks of `span` positions, one team of lanes each.  A table row with up to
+// `span` positions ("light") is added up and written by the team whose chunk it begins in, also where it ends behind
+// the chunk; the team streams through the positions with the same number of rows of g in flight whatever the rows of
+// the table they belong to.  A row with more ("hot": with popular indices one can hold a tenth of all positions) covers
+// the end of at least one chunk, so a chunk holds a part of at most two hot rows, the one it begins in and the one it
+// ends in.  The team adds up each part into a partial row, and a second kernel adds a hot row's partial rows in order.
 // ---------------------------------------------------------------------------------------------
+struct Segment {
+  int32_t from, to;  // sorted positions of one table row
+};
 struct SumArgs {
   const void *g;
   int64_t ldg;
-  const int32_t *rowptr, *key, *pos;
+  const int32_t *rowptr;  // first sorted position of every table row; nullptr after the one-launch sort, then `ends`
+  const Segment *ends;    // of every chunk: the segments of its first and of its last position
+  const int32_t *count;   // positions whose index is inside the table
+  const int32_t *key, *pos;
   int64_t rows;
-  int32_t n, d, span;
+  int32_t d, span, chunks;
   float scale, beta;
   void *out;
   int64_t ldo;
-  float *partial;  // [2 * chunks][d], float32
-  unsigned chunk_groups, chunk_teams;
+  float *partial;               // [2 * chunks][d], float32
+  int32_t *hot_count, *hot;     // parts (2 * chunk + which) that hot rows begin with, in any order
+  unsigned chunk_groups;        // workgroups that stream; those behind them write the rows that no index names
 };
 
 constexpr int kAhead = 8;  // rows of g in flight per lane
 
-// The chunk's columns of g's rows pos[from .. to), added in order.  The positions of the next kAhead rows are loaded
-// while those before them are on their way, so that a long segment pays one memory latency a step and not two.
-template <typename T>
-__device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T, true> &c, int32_t from, int32_t to,
-                                         float (&sum)[Chunk<T, true>::V]) {
+template <typename O, int V>
+__device__ __forceinline__ void put_row(const SumArgs &a, int64_t v, int32_t j, int live, float (&sum)[V]) {
+  O *out = (O *)a.out + v * a.ldo + j;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sum[i] *= a.scale;
+  if (a.beta != 0.f) {
+    float old[V];
+    load_some<O, V>(out, live, old);
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] += a.beta * old[i];
+  }
+  store_some<O, V>(out, live, sum);
+}
+
+// Adds up the chunk's columns of g's rows pos[from .. to) in order, one sum per stretch of equal keys, and hands each
+// to done(key, sum).  The positions and keys of the next kAhead rows are loaded while those before are on their way.
+template <typename T, typename F>
+__device__ __forceinline__ void stream_rows(const SumArgs &a, const Chunk<T, true> &c, int32_t from, int32_t to, F done) {
   constexpr int V = Chunk<T, true>::V;
+  if (from >= to) return;
+  int32_t p[kAhead], key[kAhead], next[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int32_t at = from + k < to ? from + k : to - 1;
+    p[k] = a.pos[at];
+    next[k] = a.key[at];
+  }
+  float sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.f;
-  if (from >= to) return;
-  int32_t p[kAhead];
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k) p[k] = a.pos[from + k < to ? from + k : to - 1];
+  int32_t now = next[0];
   for (int32_t at = from; at < to; at += kAhead) {
     Raw r[kAhead];
 #pragma unroll
@@ -276,18 +339,28 @@ __device__ __forceinline__ void add_rows(const SumArgs &a, const Chunk<T, true> 
       r[k] = Raw{0u, 0u, 0u, 0u};
       if (k == 0 || at + k < to) r[k] = c.load((const T *)a.g + (int64_t)p[k] * a.ldg);
     }
-    if (at + kAhead < to) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) p[k] = a.pos[at + kAhead + k < to ? at + kAhead + k : to - 1];
+    for (int k = 0; k < kAhead; ++k) {
+      key[k] = next[k];
+      const int32_t ahead = at + kAhead + k < to ? at + kAhead + k : to - 1;
+      p[k] = a.pos[ahead];
+      next[k] = a.key[ahead];
     }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       float f[V];
       c.floats(r[k], f);
+      if (key[k] != now) {  // never for the clamped entries behind `to`: they repeat the last key
+        done(now, sum);
+        now = key[k];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += f[i];
     }
   }
+  done(now, sum);
 }
 
 template <int DT, bool OUT_F32>
@@ -295,55 +368,59 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
   typedef typename Elem<DT>::type T;
   typedef typename Elem<OUT_F32 ? CG_F32 : DT>::type O;
   constexpr int V = Chunk<T, true>::V;
-  const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
-  const int team = threadIdx.x >> lanes_log;
-  if (blockIdx.x < a.chunk_groups) {  // parts of hot rows
-    const int32_t chunk = (int32_t)blockIdx.x * teams + team;
-    if (chunk >= (int32_t)a.chunk_teams) return;
-    const int32_t all = a.rowptr[a.rows], begin = chunk * a.span;
-    if (begin >= all) return;
-    const int32_t end = all - begin < a.span ? all : begin + a.span;
-    const int32_t first = a.key[begin], last = a.key[end - 1];
+  const int lane = threadIdx.x & ((1 << lanes_log) - 1), teams = kEmbThreads >> lanes_log, team = threadIdx.x >> lanes_log;
+  const int32_t j = ((int32_t)blockIdx.y * (1 << lanes_log) + lane) * V;
+  if (blockIdx.x >= a.chunk_groups) {  // rows without positions
+    float zero[V];
+    const int32_t left = a.d - j;
+    if (left <= 0 || a.beta == 1.f) return;
+    const int64_t step = (int64_t)(gridDim.x - a.chunk_groups) * teams;
+    for (int64_t v = (int64_t)(blockIdx.x - a.chunk_groups) * teams + team; v < a.rows; v += step)
+      if (a.rowptr[v] == a.rowptr[v + 1]) {
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const int32_t v = part == 0 ? first : last, from = a.rowptr[v], to = a.rowptr[v + 1];
-      if (to - from <= a.span || (part == 1 && first == last)) continue;
-      float *dst = a.partial + ((int64_t)chunk * 2 + part) * a.d;
-      for (int32_t j = lane * V; j < a.d; j += lanes * V) {
-        Chunk<T, true> c;
-        c.place(j, a.d);
-        float sum[V];
-        add_rows<T>(a, c, from > begin ? from : begin, to < end ? to : end, sum);
-        store_some<float, V>(dst + j, c.live, sum);
+        for (int i = 0; i < V; ++i) zero[i] = 0.f;
+        put_row<O, V>(a, v, j, left < V ? left : V, zero);
       }
-    }
     return;
   }
-  const int64_t step = (int64_t)(gridDim.x - a.chunk_groups) * teams;
-  for (int64_t v = (int64_t)(blockIdx.x - a.chunk_groups) * teams + team; v < a.rows; v += step) {
-    const int32_t from = a.rowptr[v], to = a.rowptr[v + 1];
-    if (to - from > a.span || (from == to && a.beta == 1.f)) continue;
-    O *out = (O *)a.out + v * a.ldo;
-    for (int32_t j = lane * V; j < a.d; j += lanes * V) {
-      Chunk<T, true> c;
-      c.place(j, a.d);
-      float sum[V];
-      add_rows<T>(a, c, from, to, sum);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] *= a.scale;
-      if (a.beta != 0.f) {
-        float old[V];
-        load_some<O, V>(out + j, c.live, old);
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += a.beta * old[i];
-      }
-      store_some<O, V>(out + j, c.live, sum);
+  const int32_t chunk = (int32_t)blockIdx.x * teams + team, all = *a.count;
+  if (chunk >= a.chunks || chunk * a.span >= all) return;
+  const int32_t begin = chunk * a.span, end = all - begin < a.span ? all : begin + a.span;
+  Segment first, last;
+  if (a.rowptr) {
+    const int32_t k0 = a.key[begin], k1 = a.key[end - 1];
+    first = Segment{a.rowptr[k0], a.rowptr[k0 + 1]};
+    last = Segment{a.rowptr[k1], a.rowptr[k1 + 1]};
+  } else {
+    first = a.ends[2 * chunk];
+    last = a.ends[2 * chunk + 1];
+  }
+  Chunk<T, true> c;
+  c.place(j, a.d);
+  float *partial = a.partial + (int64_t)chunk * 2 * a.d + j;
+  auto keep = [&](int32_t, float (&sum)[V]) { store_some<float, V>(partial, c.live, sum); };
+  int32_t from = begin, to = last.to;  // of the light rows that begin here
+  if (first.to - first.from > a.span) {
+    from = first.to < end ? first.to : end;
+    stream_rows<T>(a, c, begin, from, keep);
+    if (first.from == begin && lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
+  } else if (first.from < begin) {
+    from = first.to;
+  }
+  if (last.to - last.from > a.span) {
+    to = last.from;  // at or before `from` where it is the first one too
+    if (last.from > begin) {
+      partial += a.d;
+      stream_rows<T>(a, c, last.from, end, keep);
+      if (lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk + 1;
     }
   }
+  if (from < end)
+    stream_rows<T>(a, c, from, to, [&](int32_t v, float (&sum)[V]) { put_row<O, V>(a, v, j, c.live, sum); });
 }
 
-// One workgroup per chunk and 256 columns; it has work if a hot row begins in its chunk (at most one does: it covers
-// the chunk's end).  Its 16 waves take every 16th partial row each, their sums are added in order.
+// The partial rows of the hot rows, 256 columns a workgroup: its 16 wavefronts take every 16th partial row each, their
+// sums are added in order.
 constexpr int kFoldWaves = 16, kFoldColumns = kWave * 4;
 
 template <int OT>
@@ -351,47 +428,107 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
   typedef typename Elem<OT>::type O;
   __shared__ float lds[kFoldWaves][kFoldColumns];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int32_t j = blockIdx.y * kFoldColumns + lane * 4, all = a.rowptr[a.rows];
-  Chunk<float, true> c;
-  c.place(j, a.d);
-  for (int32_t chunk = blockIdx.x; chunk < (int32_t)a.chunk_teams; chunk += gridDim.x) {  // uniform in the workgroup
-    const int32_t begin = chunk * a.span;
-    if (begin >= all) return;
+  const int32_t j = blockIdx.y * kFoldColumns + lane * 4, all = *a.count, hot = *a.hot_count;
+  const int live = a.d - j < 4 ? a.d - j : 4;
+  for (int32_t h = blockIdx.x; h < hot; h += gridDim.x) {  // uniform in the workgroup
+    const int32_t chunk = a.hot[h] >> 1, which = a.hot[h] & 1, begin = chunk * a.span;
     const int32_t end = all - begin < a.span ? all : begin + a.span;
-    const int32_t v = a.key[end - 1], from = a.rowptr[v], to = a.rowptr[v + 1];
-    if (to - from <= a.span || from < begin) continue;
-    const int32_t chunks = (to - 1) / a.span - chunk + 1;
+    const int32_t v = a.key[which ? end - 1 : begin];
+    const int32_t stop = a.rowptr ? a.rowptr[v + 1] : a.ends[2 * chunk + which].to, parts = (stop - 1) / a.span - chunk + 1;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c.live > 0) {
+    if (live > 0) {
 #pragma unroll 8
-      for (int32_t k = wave; k < chunks; k += kFoldWaves) {
-        // the row's part in its first chunk is that chunk's last part unless the chunk begins with it
-        const int64_t slot = (int64_t)(chunk + k) * 2 + (k == 0 && from > begin ? 1 : 0);
+      for (int32_t k = wave; k < parts; k += kFoldWaves) {
+        const int64_t slot = (int64_t)(chunk + k) * 2 + (k == 0 ? which : 0);
         float f[4];
-        load_some<float, 4>(a.partial + slot * a.d + j, c.live, f);
+        load_some<float, 4>(a.partial + slot * a.d + j, live, f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] += f[i];
       }
     }
-    __syncthreads();  // the sums of the chunk before have been read
+    __syncthreads();  // the sums of the row before have been read
 #pragma unroll
     for (int i = 0; i < 4; ++i) lds[wave][lane * 4 + i] = sum[i];
     __syncthreads();
-    if (wave != 0 || c.live <= 0) continue;
+    if (wave != 0 || live <= 0) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum[i] = 0.f;
       for (int w = 0; w < kFoldWaves; ++w) sum[i] += lds[w][lane * 4 + i];
-      sum[i] *= a.scale;
     }
-    O *out = (O *)a.out + v * a.ldo;
-    if (a.beta != 0.f) {
-      float old[4];
-      load_some<O, 4>(out + j, c.live, old);
+    put_row<O, 4>(a, v, j, live, sum);
+  }
+}
+
+// One tile of indices: workgroup 0 sorts it in LDS and finds the chunks' first and last segments by bisection; the
+// others clear the table meanwhile (beta == 0), whose named rows the sums then overwrite.
+__device__ __forceinline__ int32_t lower_bound(const int32_t *key, int32_t n, int32_t v) {
+  int32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (key[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+template <typename O>
+__global__ __launch_bounds__(kSortThreads) void emb_small_kernel(KeySource src, int32_t n, int passes, int dbits, int32_t span,
+                                                                 int32_t *__restrict__ out_key, int32_t *__restrict__ out_pos,
+                                                                 Segment *__restrict__ ends, int32_t *__restrict__ count,
+                                                                 int32_t *__restrict__ hot_count, O *__restrict__ out,
+                                                                 int64_t ldo, int32_t d) {
+  __shared__ SortLds s;
+  if (blockIdx.x > 0) {
+    constexpr int V = 16 / (int)sizeof(O);
+    const int32_t per_row = (d + V - 1) / V;
+    const int64_t units = src.rows * per_row, step = (int64_t)(gridDim.x - 1) * kSortThreads;
+    float zero[V];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] += a.beta * old[i];
+    for (int i = 0; i < V; ++i) zero[i] = 0.f;
+    for (int64_t u = (int64_t)(blockIdx.x - 1) * kSortThreads + threadIdx.x; u < units; u += step) {
+      const int64_t row = u / per_row;
+      const int32_t j = (int32_t)(u - row * per_row) * V;
+      store_some<O, V>(out + row * ldo + j, d - j < V ? d - j : V, zero);
     }
-    store_some<O, 4>(out + j, c.live, sum);
+    return;
+  }
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  int32_t key[kKeysPerLane], pos[kKeysPerLane];
+  int at[kKeysPerLane];
+#pragma unroll
+  for (int r = 0; r < kKeysPerLane; ++r) {
+    const int i = wave * kWaveKeys + r * kWave + lane;
+    at[r] = i < n ? i : n - 1;
+    key[r] = key_at(src, at[r]);
+    pos[r] = at[r];
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    if (pass > 0) {
+#pragma unroll
+      for (int r = 0; r < kKeysPerLane; ++r) {
+        key[r] = s.key[at[r]];
+        pos[r] = s.pos[at[r]];
+      }
+      __syncthreads();
+    }
+    (void)sort_tile(s, key, pos, n, pass * dbits, dbits);
+  }
+  for (int i = threadIdx.x; i < n; i += kSortThreads) {
+    out_key[i] = s.key[i];
+    out_pos[i] = s.pos[i];
+  }
+  const int32_t all = lower_bound(s.key, n, (int32_t)src.rows);
+  if (threadIdx.x == 0) {
+    *count = all;
+    *hot_count = 0;
+  }
+  for (int32_t e = threadIdx.x; (e >> 1) * span < all; e += kSortThreads) {
+    const int32_t begin = (e >> 1) * span, end = all - begin < span ? all : begin + span;
+    const int32_t v = s.key[(e & 1) ? end - 1 : begin];
+    ends[e] = Segment{lower_bound(s.key, n, v), lower_bound(s.key, n, v + 1)};
   }
 }
 
@@ -400,14 +537,14 @@ struct EmbPlan {
   int passes, dbits;
   int64_t tiles, chunks;
   int32_t span;
-  size_t key[2], pos[2], hist, totals, rowptr, partial, bytes;  // offsets into the workspace
+  size_t key[2], pos[2], hist, totals, rowptr, ends, counters, hot, partial, bytes;  // offsets into the workspace
 };
 static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   EmbPlan p = {};
-  int bits = bits_for((int32_t)(rows + 1));
-  p.passes = bits > 0 ? (bits + kMaxDigit - 1) / kMaxDigit : 1;
-  p.dbits = bits > 0 ? (bits + p.passes - 1) / p.passes : 1;
-  p.tiles = ceil_div64(n, kEmbTile);
+  const int bits = bits_for((int32_t)(rows + 1));
+  p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
+  p.dbits = (bits + p.passes - 1) / p.passes;
+  p.tiles = ceil_div64(n, kSortTile);
   // about sqrt(n / 128): the longest chain of additions in a team and the longest list of partial rows grow alike
   p.span = 32;
   while (p.span < 512 && (int64_t)p.span * p.span * 128 < n) p.span *= 2;
@@ -422,6 +559,9 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.hist = take((size_t)p.tiles * ((size_t)1 << p.dbits) * 4);
   p.totals = take((size_t)kMaxRadix * 4);
   p.rowptr = take((size_t)(rows + 2) * 4);
+  p.ends = take(p.tiles <= 1 ? (size_t)p.chunks * 2 * sizeof(Segment) : 0);
+  p.counters = take(8);  // positions inside the table, hot rows
+  p.hot = take((size_t)p.chunks * 4);
   p.partial = take((size_t)p.chunks * 2 * (size_t)d * 4);
   p.bytes = at;
   return p;
@@ -430,6 +570,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
 static int check_lookup(const char *who, int64_t n, int64_t rows, int32_t d) {
   if (n < 0 || rows <= 0 || d <= 0)
     CG_FAIL(CG_ERR_SIZE, "%s: n=%lld indices into rows=%lld of d=%d elements", who, (long long)n, (long long)rows, d);
+  if (d > (1 << 23)) CG_FAIL(CG_ERR_OVERFLOW, "%s: rows of d=%d elements (at most 2^23)", who, d);
   if (n > 0x7fff0000LL || rows > 0x7ffffffdLL)
     CG_FAIL(CG_ERR_OVERFLOW, "%s: n=%lld, rows=%lld overflow int32 positions", who, (long long)n, (long long)rows);
   return CG_OK;
@@ -492,41 +633,67 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   int32_t *key[2] = {(int32_t *)(w + p.key[0]), (int32_t *)(w + p.key[1])};
   int32_t *pos[2] = {(int32_t *)(w + p.pos[0]), (int32_t *)(w + p.pos[1])};
   uint32_t *hist = (uint32_t *)(w + p.hist), *totals = (uint32_t *)(w + p.totals);
-  int32_t *rowptr = (int32_t *)(w + p.rowptr);
-  int last = 0;
-  if (n > 0) {
-    KeySource src = {{d_idx, idx64 != 0}, nullptr, nullptr, rows};
-    for (int pass = 0; pass < p.passes; ++pass) {
-      const int to = pass & 1, shift = pass * p.dbits, radix = 1 << p.dbits;
-      emb_hist_kernel<<<(unsigned)p.tiles, kEmbThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles);
+  int32_t *rowptr = (int32_t *)(w + p.rowptr), *counters = (int32_t *)(w + p.counters);
+  SumArgs a = {};
+  a.g = d_g, a.ldg = ldg, a.count = counters, a.rows = rows, a.d = d, a.span = p.span, a.chunks = (int32_t)p.chunks;
+  a.scale = scale, a.beta = beta, a.out = d_out, a.ldo = ldo, a.partial = (float *)(w + p.partial);
+  a.hot_count = counters + 1, a.hot = (int32_t *)(w + p.hot);
+  KeySource src = {{d_idx, idx64 != 0}, nullptr, nullptr, rows};
+  const bool small = n > 0 && p.tiles <= 1 && (beta == 0.f || beta == 1.f);
+  if (small) {
+    Segment *ends = (Segment *)(w + p.ends);
+    const int64_t units = beta == 0.f ? rows * ceil_div64(d, out_dtype == CG_F32 ? 4 : 8) : 0;
+    int64_t groups = ceil_div64(units, kSortThreads * 4);
+    groups = 1 + (groups < 1024 ? groups : 1024);
+#define CG_CALL(OT)                                                                                                     \
+  emb_small_kernel<<<(unsigned)groups, kSortThreads, 0, s>>>(src, (int32_t)n, p.passes, p.dbits, p.span, key[0], pos[0], ends, \
+                                                             counters, counters + 1, (Elem<OT>::type *)d_out, ldo, d)
+    CG_BY_DTYPE(out_dtype, CG_CALL)
+#undef CG_CALL
+    CG_LAUNCH_CHECK();
+    a.key = key[0], a.pos = pos[0], a.ends = ends;
+  } else {
+    int last = 0;
+    const bool direct = p.tiles <= kDirectTiles;
+    const int radix = 1 << p.dbits;
+    for (int pass = 0; n > 0 && pass < p.passes; ++pass) {
+      const int to = pass & 1, shift = pass * p.dbits;
+      emb_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, direct ? 1 : p.tiles,
+                                                                 direct ? radix : 1);
       CG_LAUNCH_CHECK();
-      emb_scan_kernel<<<(unsigned)ceil_div64(radix, kEmbWaves), kEmbThreads, 0, s>>>(hist, p.tiles, radix, totals);
-      CG_LAUNCH_CHECK();
-      emb_scatter_kernel<<<(unsigned)p.tiles, kEmbThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals, key[to], pos[to]);
+      if (direct) {
+        emb_scatter_kernel<true><<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals,
+                                                                            key[to], pos[to], counters + 1);
+      } else {
+        emb_scan_kernel<<<(unsigned)ceil_div64(radix, kEmbWaves), kEmbThreads, 0, s>>>(hist, p.tiles, radix, totals);
+        CG_LAUNCH_CHECK();
+        emb_scatter_kernel<false><<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals,
+                                                                             key[to], pos[to], counters + 1);
+      }
       CG_LAUNCH_CHECK();
       src.key = key[to], src.pos = pos[to];
       last = to;
     }
+    CG_TRY(launch_rowptr(key[last], n, (int32_t)(rows + 1), rowptr, s));
+    a.key = key[last], a.pos = pos[last], a.rowptr = rowptr, a.count = rowptr + rows;
   }
-  CG_TRY(launch_rowptr(key[last], n, (int32_t)(rows + 1), rowptr, s));
-  const int lanes_log = lanes_log2(d, dtype == CG_F32 ? 4 : 8), teams = kEmbThreads >> lanes_log;
-  SumArgs a = {};
-  a.g = d_g, a.ldg = ldg, a.rowptr = rowptr, a.key = key[last], a.pos = pos[last], a.rows = rows, a.n = (int32_t)n, a.d = d;
-  a.span = p.span, a.scale = scale, a.beta = beta, a.out = d_out, a.ldo = ldo, a.partial = (float *)(w + p.partial);
-  a.chunk_teams = (unsigned)p.chunks, a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
-  int64_t groups = ceil_div64(rows, teams);
-  if (groups > 256 * 64) groups = 256 * 64;
+  const int per_chunk = dtype == CG_F32 ? 4 : 8, lanes_log = lanes_log2(d, per_chunk), teams = kEmbThreads >> lanes_log;
+  a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
+  int64_t groups = small || beta == 1.f ? 0 : ceil_div64(rows, teams);
+  if (groups > 256 * 16) groups = 256 * 16;
   groups += a.chunk_groups;
-#define CG_CALL(DT)                                                                  \
-  if (out_dtype == CG_F32)                                                           \
-    emb_sum_kernel<DT, true><<<(unsigned)groups, kEmbThreads, 0, s>>>(a, lanes_log); \
-  else                                                                               \
-    emb_sum_kernel<DT, false><<<(unsigned)groups, kEmbThreads, 0, s>>>(a, lanes_log)
+  if (groups == 0) return CG_OK;
+  const dim3 grid((unsigned)groups, (unsigned)ceil_div64(d, (int64_t)per_chunk << lanes_log));
+#define CG_CALL(DT)                                                      \
+  if (out_dtype == CG_F32)                                               \
+    emb_sum_kernel<DT, true><<<grid, kEmbThreads, 0, s>>>(a, lanes_log); \
+  else                                                                   \
+    emb_sum_kernel<DT, false><<<grid, kEmbThreads, 0, s>>>(a, lanes_log)
   CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();
   if (n <= p.span) return CG_OK;  // no row can be hot
-  const dim3 fold((unsigned)(p.chunks < 65536 ? p.chunks : 65536), (unsigned)ceil_div64(d, kFoldColumns));
+  const dim3 fold((unsigned)(p.chunks < 512 ? p.chunks : 512), (unsigned)ceil_div64(d, kFoldColumns));
 #define CG_CALL(OT) emb_fold_kernel<OT><<<fold, kWave * kFoldWaves, 0, s>>>(a)
   CG_BY_DTYPE(out_dtype, CG_CALL)
 #undef CG_CALL
