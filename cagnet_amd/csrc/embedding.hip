@@ -545,9 +545,9 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   p.dbits = (bits + p.passes - 1) / p.passes;
   p.tiles = ceil_div64(n, kSortTile);
-  // about sqrt(n / 128): the longest chain of additions in a team and the longest list of partial rows grow alike
+  // about sqrt(n / 512): the longest chain of additions in a team and the longest list of partial rows grow alike
   p.span = 32;
-  while (p.span < 512 && (int64_t)p.span * p.span * 128 < n) p.span *= 2;
+  while (p.span < 512 && (int64_t)p.span * p.span * 512 < n) p.span *= 2;
   p.chunks = ceil_div64(n, p.span);
   size_t at = 0;
   auto take = [&at](size_t bytes) {

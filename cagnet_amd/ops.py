@@ -636,26 +636,22 @@ def log_softmax_nll_bwd(logp: torch.Tensor, y: torch.Tensor, mask: Optional[torc
 _ROW_DTYPES = {torch.float32: _lib.CG_F32, torch.bfloat16: _lib.CG_BF16, torch.float16: _lib.CG_F16}
 
 
-class _On:
-    """The device and stream a call runs on: those of its operands, whatever device is current."""
+# torch.cuda.current_device() and current_stream() build Python objects; a call on a few thousand rows is bound by the
+# host (about 3 us of kernel against 10 us of Python), so the raw handles are taken from underneath them.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    __slots__ = ("device", "guard", "stream")
 
-    def __init__(self, t: torch.Tensor):
-        self.device = t.device
-        self.guard = None
-
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _run(device: torch.device, where: str, fn, *args) -> None:
+    """fn(*args, stream) on the operands' device and its current stream, whatever device is current."""
+    index = device.index
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, where)
 
 
 def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, int]:
@@ -665,23 +661,26 @@ def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> Tu
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"{name}: must live on the GPU (got device {t.device}); there is no CPU path")
+    shape = t.shape
     if like is not None:
         if t.dtype != like.dtype:
             raise TypeError(f"{name}: expected dtype {like.dtype}, got {t.dtype}")
-        if t.shape != like.shape:
-            raise ValueError(f"{name}: expected shape {tuple(like.shape)}, got {tuple(t.shape)}")
+        if shape != like.shape:
+            raise ValueError(f"{name}: expected shape {tuple(like.shape)}, got {tuple(shape)}")
         if t.device != like.device:
             raise ValueError(f"{name}: on {t.device}, the other operands are on {like.device}")
     elif t.dtype not in _ROW_DTYPES:
         raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    elif t.dim() != 2:
-        raise ValueError(f"{name}: expected 2 dimensions, got {t.dim()}")
-    rows, cols = t.shape
+    elif len(shape) != 2:
+        raise ValueError(f"{name}: expected 2 dimensions, got {len(shape)}")
+    rows, cols = shape
     if cols == 0:
         raise ValueError(f"{name}: rows of no elements")
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    ld, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and ld < cols):
         t = t.contiguous()
-    return t, max(t.stride(0) if rows > 1 else cols, cols)
+        ld = cols
+    return t, ld if rows > 1 and ld > cols else cols
 
 
 def _weights(x: torch.Tensor, **named: Optional[torch.Tensor]):
@@ -754,9 +753,8 @@ def rng_next(state: torch.Tensor) -> torch.Tensor:
     """A snapshot of `state` for one dropout (its forward pass and its gradient), and `state` steps on."""
     state = _need_rng(state, "state")
     snapshot = torch.empty_like(state)
-    with _On(state) as on:
-        torch.autograd.graph.increment_version(state)
-        check(lib.cg_rng_next(state.data_ptr(), snapshot.data_ptr(), on.stream), "cg_rng_next")
+    torch.autograd.graph.increment_version(state)
+    _run(state.device, "cg_rng_next", lib.cg_rng_next, state.data_ptr(), snapshot.data_ptr())
     return snapshot
 
 
@@ -765,9 +763,7 @@ def _dropout(x: torch.Tensor, p: float, rng: Optional[torch.Tensor], name: str) 
     p = _probability(p, rng, x)
     n, d = x.shape
     out = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    with _On(x) as on:
-        check(lib.cg_dropout(x.data_ptr(), ldx, out.data_ptr(), d, n, d, _ROW_DTYPES[x.dtype], p, _at(rng), on.stream),
-              "cg_dropout")
+    _run(x.device, "cg_dropout", lib.cg_dropout, x.data_ptr(), ldx, out.data_ptr(), d, n, d, _ROW_DTYPES[x.dtype], p, _at(rng))
     return out
 
 
@@ -801,10 +797,8 @@ def embedding_fwd(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) ->
     rows, d = table.shape
     n = idx.shape[0]
     out = torch.empty((n, d), dtype=table.dtype, device=table.device)
-    with _On(table) as on:
-        check(lib.cg_embedding_fwd(table.data_ptr(), ldt, rows, idx.data_ptr(), int(idx.dtype == torch.int64), n, d,
-                                   _ROW_DTYPES[table.dtype], float(scale), out.data_ptr(), d, on.stream),
-              "cg_embedding_fwd")
+    _run(table.device, "cg_embedding_fwd", lib.cg_embedding_fwd, table.data_ptr(), ldt, rows, idx.data_ptr(),
+         idx.dtype == torch.int64, n, d, _ROW_DTYPES[table.dtype], scale, out.data_ptr(), d)
     return out
 
 
@@ -834,10 +828,9 @@ def embedding_bwd(g: torch.Tensor, idx: torch.Tensor, rows: int, scale: float = 
         torch.autograd.graph.increment_version(out)
     ldo = max(out.stride(0) if rows > 1 else d, d)
     work = _workspace(lib.cg_embedding_bwd_workspace, "cg_embedding_bwd_workspace", g.device, n, rows, d)
-    with _On(g) as on:
-        check(lib.cg_embedding_bwd(g.data_ptr(), ldg, idx.data_ptr(), int(idx.dtype == torch.int64), n, rows, d,
-                                   _ROW_DTYPES[g.dtype], _ROW_DTYPES[out.dtype], float(scale), float(beta),
-                                   out.data_ptr(), ldo, work.data_ptr(), work.numel(), on.stream), "cg_embedding_bwd")
+    _run(g.device, "cg_embedding_bwd", lib.cg_embedding_bwd, g.data_ptr(), ldg, idx.data_ptr(), idx.dtype == torch.int64, n,
+         rows, d, _ROW_DTYPES[g.dtype], _ROW_DTYPES[out.dtype], scale, beta, out.data_ptr(), ldo, work.data_ptr(),
+         work.numel())
     return out
 
 
@@ -848,9 +841,8 @@ def rms_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1
     n, d = x.shape
     y = torch.empty((n, d), dtype=x.dtype, device=x.device)
     rstd = torch.empty(n, dtype=torch.float32, device=x.device)
-    with _On(x) as on:
-        check(lib.cg_rms_norm_fwd(x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], y.data_ptr(), d, rstd.data_ptr(), n, d,
-                                  _ROW_DTYPES[x.dtype], float(eps), on.stream), "cg_rms_norm_fwd")
+    _run(x.device, "cg_rms_norm_fwd", lib.cg_rms_norm_fwd, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], y.data_ptr(), d,
+         rstd.data_ptr(), n, d, _ROW_DTYPES[x.dtype], eps)
     return y, rstd
 
 
@@ -864,10 +856,8 @@ def rms_norm_bwd(g: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor
     dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
     dw = torch.empty_like(w) if w is not None else None
     work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", x.device, n, d)
-    with _On(x) as on:
-        check(lib.cg_rms_norm_bwd(g.data_ptr(), ldg, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], rstd.data_ptr(),
-                                  dx.data_ptr(), d, _at(dw), n, d, _ROW_DTYPES[x.dtype], work.data_ptr(), work.numel(),
-                                  on.stream), "cg_rms_norm_bwd")
+    _run(x.device, "cg_rms_norm_bwd", lib.cg_rms_norm_bwd, g.data_ptr(), ldg, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype],
+         rstd.data_ptr(), dx.data_ptr(), d, _at(dw), n, d, _ROW_DTYPES[x.dtype], work.data_ptr(), work.numel())
     return dx, dw
 
 
@@ -900,11 +890,9 @@ def norm_residual_fwd(z: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.T
     h = torch.empty_like(r)
     rstd_z = torch.empty(n, dtype=torch.float32, device=z.device)
     rstd_r = torch.empty_like(rstd_z)
-    with _On(z) as on:
-        check(lib.cg_norm_residual_fwd(z.data_ptr(), ldz, x.data_ptr(), ldx, _at(gate), ldg, kind, _at(w_post), _at(w_pre),
-                                       _at(scale), _ROW_DTYPES[wdtype], float(alpha), p, _at(rng), float(eps),
-                                       r.data_ptr(), d, h.data_ptr(), d, rstd_z.data_ptr(), rstd_r.data_ptr(), n, d,
-                                       _ROW_DTYPES[z.dtype], on.stream), "cg_norm_residual_fwd")
+    _run(z.device, "cg_norm_residual_fwd", lib.cg_norm_residual_fwd, z.data_ptr(), ldz, x.data_ptr(), ldx, _at(gate), ldg,
+         kind, _at(w_post), _at(w_pre), _at(scale), _ROW_DTYPES[wdtype], alpha, p, _at(rng), eps, r.data_ptr(), d,
+         h.data_ptr(), d, rstd_z.data_ptr(), rstd_r.data_ptr(), n, d, _ROW_DTYPES[z.dtype])
     return r, h, rstd_z, rstd_r
 
 
@@ -933,13 +921,11 @@ def norm_residual_bwd(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], z:
     dgate = torch.empty(gate.shape, dtype=z.dtype, device=z.device) if gate is not None else None
     dw_post, dw_pre, dscale = (torch.empty_like(w) if w is not None else None for w in (w_post, w_pre, scale))
     work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", z.device, n, d)
-    with _On(z) as on:
-        check(lib.cg_norm_residual_bwd(_at(dr), lddr, _at(dh), lddh, z.data_ptr(), ldz, r.data_ptr(), ldr, _at(gate), ldg,
-                                       kind, _at(w_post), _at(w_pre), _at(scale), _ROW_DTYPES[wdtype], float(alpha), p,
-                                       _at(rng), rstd_z.data_ptr(), rstd_r.data_ptr(), dz.data_ptr(), d, dx.data_ptr(), d,
-                                       _at(dgate), dgate.shape[1] if dgate is not None else 0, _at(dw_post), _at(dw_pre),
-                                       _at(dscale), n, d, _ROW_DTYPES[z.dtype], work.data_ptr(), work.numel(), on.stream),
-              "cg_norm_residual_bwd")
+    _run(z.device, "cg_norm_residual_bwd", lib.cg_norm_residual_bwd, _at(dr), lddr, _at(dh), lddh, z.data_ptr(), ldz,
+         r.data_ptr(), ldr, _at(gate), ldg, kind, _at(w_post), _at(w_pre), _at(scale), _ROW_DTYPES[wdtype], alpha, p,
+         _at(rng), rstd_z.data_ptr(), rstd_r.data_ptr(), dz.data_ptr(), d, dx.data_ptr(), d, _at(dgate),
+         dgate.shape[1] if dgate is not None else 0, _at(dw_post), _at(dw_pre), _at(dscale), n, d, _ROW_DTYPES[z.dtype],
+         work.data_ptr(), work.numel())
     return dz, dx, dgate, dw_post, dw_pre, dscale
 
 
