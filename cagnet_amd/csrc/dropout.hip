@@ -13,29 +13,63 @@ __global__ void rng_next_kernel(int64_t *__restrict__ state, int64_t *__restrict
   state[1] = (int64_t)((uint64_t)off + 1ull);
 }
 
-// One thread per four consecutive columns: one generator call decides them.
-template <int DT>
+// 16 bytes a thread and step: one generator call for four float32 columns, two for eight 16-bit ones.  Threads walk the
+// chunks of the whole array in order, `rows_on` rows and `chunks_on` chunks further at every step.  kSteps chunks are
+// loaded before the first is decided: their generator calls run while the loads are on their way.
+constexpr int kSteps = 2;
+
+template <int DT, bool RAGGED>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const typename Elem<DT>::type *x, int64_t ldx,
                                                                typename Elem<DT>::type *out, int64_t ldo, int64_t n,
-                                                               int32_t d, Mask m) {
-  const int32_t blocks = (d + 3) / 4;
-  const int64_t total = n * blocks, step = (int64_t)gridDim.x * kDropThreads;
+                                                               int32_t d, int32_t chunks, int64_t rows_on,
+                                                               int32_t chunks_on, Mask m) {
+  typedef typename Elem<DT>::type T;
+  typedef Chunk<T, RAGGED> C;
   MaskKey key = {0, 0, 0, 0};
   if (m.rng) key = mask_key(m.rng);
-  for (int64_t i = (int64_t)blockIdx.x * kDropThreads + threadIdx.x; i < total; i += step) {
-    const int64_t row = i / blocks;
-    const int32_t block = (int32_t)(i - row * blocks), j = block * 4;
-    const int live = d - j < 4 ? d - j : 4;
-    float v[4];
-    load_some(x + row * ldx + j, live, v);
-    if (m.rng) {
-      uint32_t w[4];
-      mask_words(key, (uint32_t)row, (uint32_t)block, w);
+  const int64_t first = (int64_t)blockIdx.x * kDropThreads + threadIdx.x;
+  int64_t row = first / chunks;
+  int32_t at = (int32_t)(first - row * chunks);
+  while (row < n) {
+    C c[kSteps];
+    Raw r[kSteps];
+    int64_t rows[kSteps];
+    int32_t cols[kSteps];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = w[k] > m.last ? v[k] * m.inv_keep : 0.f;
+    for (int k = 0; k < kSteps; ++k) {
+      rows[k] = row;
+      cols[k] = at;
+      c[k].place(at * C::V, d);
+      r[k] = c[k].load(x + (row < n ? row : n - 1) * ldx);
+      row += rows_on;
+      at += chunks_on;
+      if (at >= chunks) at -= chunks, ++row;
     }
-    store_some(out + row * ldo + j, live, v);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      float v[C::V];
+      c[k].floats(r[k], v);
+      if (m.rng) drop_chunk<C::V>(key, m, rows[k], cols[k] * C::V, v);
+      if (rows[k] < n) c[k].write(out + rows[k] * ldo, v);
+    }
   }
+}
+
+template <int DT>
+static void launch_dropout(const void *x, int64_t ldx, void *out, int64_t ldo, int64_t n, int32_t d, const Mask &m,
+                           hipStream_t s) {
+  typedef typename Elem<DT>::type T;
+  const int v = Chunk<T, false>::V;
+  const int32_t chunks = (int32_t)ceil_div64(d, v);
+  int64_t groups = ceil_div64(n * chunks, kDropThreads * kSteps);
+  if (groups > 256 * 128) groups = 256 * 128;
+  const int64_t step = groups * kDropThreads;
+  if (d % v == 0)
+    dropout_kernel<DT, false><<<(unsigned)groups, kDropThreads, 0, s>>>((const T *)x, ldx, (T *)out, ldo, n, d, chunks,
+                                                                        step / chunks, (int32_t)(step % chunks), m);
+  else
+    dropout_kernel<DT, true><<<(unsigned)groups, kDropThreads, 0, s>>>((const T *)x, ldx, (T *)out, ldo, n, d, chunks,
+                                                                       step / chunks, (int32_t)(step % chunks), m);
 }
 
 }  // namespace cg
@@ -64,11 +98,7 @@ int cg_dropout(const void *d_x, int64_t ldx, void *d_out, int64_t ldo, int64_t n
   const Mask m = make_mask(p, d_rng);
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof("dropout", d, s);
-  int64_t groups = ceil_div64(n * ((d + 3) / 4), kDropThreads);
-  if (groups > 256 * 64) groups = 256 * 64;
-#define CG_CALL(DT)                                                                                                    \
-  dropout_kernel<DT><<<(unsigned)groups, kDropThreads, 0, s>>>((const Elem<DT>::type *)d_x, ldx, (Elem<DT>::type *)d_out, \
-                                                               ldo, n, d, m)
+#define CG_CALL(DT) launch_dropout<DT>(d_x, ldx, d_out, ldo, n, d, m, s)
   CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();

@@ -173,6 +173,8 @@ __device__ __forceinline__ uint32_t sort_tile(SortLds &s, const int32_t (&key)[k
   const uint64_t below = (1ull << lane) - 1ull;
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r) {
+    rank[r] = 0;
+    if (wave * kWaveKeys + r * kWave >= here) continue;  // the whole wavefront is behind the last key
     const bool valid = wave * kWaveKeys + r * kWave + lane < here;
     const uint32_t digit = ((uint32_t)key[r] >> shift) & (uint32_t)(radix - 1);
     uint64_t peers = __ballot(valid);
@@ -191,18 +193,20 @@ __device__ __forceinline__ uint32_t sort_tile(SortLds &s, const int32_t (&key)[k
     rank[r] = had + lower;
   }
   __syncthreads();
-  uint32_t mine = 0;
+  uint32_t mine = 0, of[kSortWaves];
+  const int digit_of = (int)threadIdx.x & (radix - 1);
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) of[w] = s.count[w][digit_of];
   if ((int)threadIdx.x < radix)
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) mine += s.count[w][threadIdx.x];
+    for (int w = 0; w < kSortWaves; ++w) mine += of[w];
   const uint32_t first = group_exclusive(mine, s.wave_sums);
   if ((int)threadIdx.x < radix) {
     uint32_t run = first;
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = s.count[w][threadIdx.x];
       s.count[w][threadIdx.x] = run;
-      run += c;
+      run += of[w];
     }
   }
   __syncthreads();
@@ -462,14 +466,24 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
 
 // One tile of indices: workgroup 0 sorts it in LDS and finds the chunks' first and last segments by bisection; the
 // others clear the table meanwhile (beta == 0), whose named rows the sums then overwrite.
-__device__ __forceinline__ int32_t lower_bound(const int32_t *key, int32_t n, int32_t v) {
-  int32_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (key[mid] < v)
-      lo = mid + 1;
-    else
-      hi = mid;
+// first place of a key not below v, and of one above it
+__device__ __forceinline__ Segment segment_of(const int32_t *key, int32_t n, int32_t v) {
+  Segment lo = {0, 0}, hi = {n, n};
+  while (lo.from < hi.from || lo.to < hi.to) {  // both bisections side by side: each step is an LDS round trip
+    const int32_t m = (lo.from + hi.from) >> 1, k = (lo.to + hi.to) >> 1;
+    const int32_t km = key[m < n ? m : n - 1], kk = key[k < n ? k : n - 1];
+    if (lo.from < hi.from) {
+      if (km < v)
+        lo.from = m + 1;
+      else
+        hi.from = m;
+    }
+    if (lo.to < hi.to) {
+      if (kk <= v)
+        lo.to = k + 1;
+      else
+        hi.to = k;
+    }
   }
   return lo;
 }
@@ -520,7 +534,7 @@ __global__ __launch_bounds__(kSortThreads) void emb_small_kernel(KeySource src, 
     out_key[i] = s.key[i];
     out_pos[i] = s.pos[i];
   }
-  const int32_t all = lower_bound(s.key, n, (int32_t)src.rows);
+  const int32_t all = segment_of(s.key, n, (int32_t)src.rows).from;
   if (threadIdx.x == 0) {
     *count = all;
     *hot_count = 0;
@@ -528,7 +542,7 @@ __global__ __launch_bounds__(kSortThreads) void emb_small_kernel(KeySource src, 
   for (int32_t e = threadIdx.x; (e >> 1) * span < all; e += kSortThreads) {
     const int32_t begin = (e >> 1) * span, end = all - begin < span ? all : begin + span;
     const int32_t v = s.key[(e & 1) ? end - 1 : begin];
-    ends[e] = Segment{lower_bound(s.key, n, v), lower_bound(s.key, n, v + 1)};
+    ends[e] = segment_of(s.key, n, v);
   }
 }
 
@@ -545,9 +559,9 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   p.dbits = (bits + p.passes - 1) / p.passes;
   p.tiles = ceil_div64(n, kSortTile);
-  // about sqrt(n / 512): the longest chain of additions in a team and the longest list of partial rows grow alike
-  p.span = 32;
-  while (p.span < 512 && (int64_t)p.span * p.span * 512 < n) p.span *= 2;
+  // about sqrt(n / 256): the longest chain of additions in a team and the longest list of partial rows grow alike
+  p.span = 8;
+  while (p.span < 512 && (int64_t)p.span * p.span * 256 < n) p.span *= 2;
   p.chunks = ceil_div64(n, p.span);
   size_t at = 0;
   auto take = [&at](size_t bytes) {

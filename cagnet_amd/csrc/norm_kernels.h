@@ -90,16 +90,4 @@ __device__ __forceinline__ void weight_chunk(const void *w, int w_f32, int32_t j
   for (int i = 0; i < V; ++i) out[i] = i < live ? weight_at<T>(w, w_f32, j + i) : 0.f;
 }
 
-// v / (1 - p) for the kept elements of the chunk that starts at column j (a multiple of four), 0 for the others
-template <int V>
-__device__ __forceinline__ void drop_chunk(const MaskKey &k, const Mask &m, int64_t row, int32_t j, float (&v)[V]) {
-#pragma unroll
-  for (int b = 0; b < V / 4; ++b) {
-    uint32_t w[4];
-    mask_words(k, (uint32_t)row, (uint32_t)(j / 4 + b), w);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[4 * b + i] = w[i] > m.last ? v[4 * b + i] * m.inv_keep : 0.f;
-  }
-}
-
 }  // namespace cg

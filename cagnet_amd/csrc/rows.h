@@ -191,14 +191,19 @@ __device__ __forceinline__ MaskKey mask_key(const int64_t *__restrict__ rng) {
   return MaskKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
 }
 
+// one instruction with the truth table of a ^ b ^ c
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 // the four words of columns 4 * block .. 4 * block + 3 of `row`
 __device__ __forceinline__ void mask_words(const MaskKey &k, uint32_t row, uint32_t block, uint32_t (&w)[4]) {
   uint32_t c0 = block, c1 = row, c2 = k.off_lo, c3 = k.off_hi, k0 = k.seed_lo, k1 = k.seed_hi;
 #pragma unroll
   for (int r = 0; r < kPhiloxRounds; ++r) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c1 = (uint32_t)b;
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
@@ -215,6 +220,18 @@ __device__ __forceinline__ float mask_at(const MaskKey &k, const Mask &m, int64_
   mask_words(k, (uint32_t)row, (uint32_t)j >> 2, w);
   const uint32_t mine = (j & 2) ? ((j & 1) ? w[3] : w[2]) : ((j & 1) ? w[1] : w[0]);
   return mine > m.last ? m.inv_keep : 0.f;
+}
+
+// v / (1 - p) for the kept elements of the chunk that starts at column j (a multiple of four), 0 for the others
+template <int V>
+__device__ __forceinline__ void drop_chunk(const MaskKey &k, const Mask &m, int64_t row, int32_t j, float (&v)[V]) {
+#pragma unroll
+  for (int b = 0; b < V / 4; ++b) {
+    uint32_t w[4];
+    mask_words(k, (uint32_t)row, (uint32_t)(j / 4 + b), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[4 * b + i] = w[i] > m.last ? v[4 * b + i] * m.inv_keep : 0.f;
+  }
 }
 
 // ---- argument checks shared by the entry points ---------------------------------------------------

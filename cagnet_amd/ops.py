@@ -8,6 +8,7 @@ training operators (dropout, embedding, rms_norm, norm_residual) also take bfloa
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_int64, c_void_p
 from typing import Optional, Sequence, Tuple
 
@@ -736,10 +737,15 @@ def _need_rng(rng: torch.Tensor, name: str, device=None) -> torch.Tensor:
     return rng
 
 
-def _workspace(query, where: str, device, *sizes) -> torch.Tensor:
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, *sizes: int) -> int:
     need = ctypes.c_int64(0)
-    check(query(*sizes, ctypes.byref(need)), where)
-    return torch.empty(max(need.value, 16), dtype=torch.uint8, device=device)
+    check(getattr(lib, query)(*sizes, ctypes.byref(need)), query)
+    return max(need.value, 16)
+
+
+def _workspace(query: str, device, *sizes: int) -> torch.Tensor:
+    return torch.empty(_workspace_bytes(query, *sizes), dtype=torch.uint8, device=device)
 
 
 def rng_state(seed: int, device="cuda:0", offset: int = 0) -> torch.Tensor:
@@ -827,7 +833,7 @@ def embedding_bwd(g: torch.Tensor, idx: torch.Tensor, rows: int, scale: float = 
             raise ValueError(f"out: output must be row-major with unit column stride (strides {out.stride()})")
         torch.autograd.graph.increment_version(out)
     ldo = max(out.stride(0) if rows > 1 else d, d)
-    work = _workspace(lib.cg_embedding_bwd_workspace, "cg_embedding_bwd_workspace", g.device, n, rows, d)
+    work = _workspace("cg_embedding_bwd_workspace", g.device, n, rows, d)
     _run(g.device, "cg_embedding_bwd", lib.cg_embedding_bwd, g.data_ptr(), ldg, idx.data_ptr(), idx.dtype == torch.int64, n,
          rows, d, _ROW_DTYPES[g.dtype], _ROW_DTYPES[out.dtype], scale, beta, out.data_ptr(), ldo, work.data_ptr(),
          work.numel())
@@ -855,7 +861,7 @@ def rms_norm_bwd(g: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor
     n, d = x.shape
     dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
     dw = torch.empty_like(w) if w is not None else None
-    work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", x.device, n, d)
+    work = _workspace("cg_norm_bwd_workspace", x.device, n, d)
     _run(x.device, "cg_rms_norm_bwd", lib.cg_rms_norm_bwd, g.data_ptr(), ldg, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype],
          rstd.data_ptr(), dx.data_ptr(), d, _at(dw), n, d, _ROW_DTYPES[x.dtype], work.data_ptr(), work.numel())
     return dx, dw
@@ -920,7 +926,7 @@ def norm_residual_bwd(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], z:
     dx = torch.empty_like(dz)
     dgate = torch.empty(gate.shape, dtype=z.dtype, device=z.device) if gate is not None else None
     dw_post, dw_pre, dscale = (torch.empty_like(w) if w is not None else None for w in (w_post, w_pre, scale))
-    work = _workspace(lib.cg_norm_bwd_workspace, "cg_norm_bwd_workspace", z.device, n, d)
+    work = _workspace("cg_norm_bwd_workspace", z.device, n, d)
     _run(z.device, "cg_norm_residual_bwd", lib.cg_norm_residual_bwd, _at(dr), lddr, _at(dh), lddh, z.data_ptr(), ldz,
          r.data_ptr(), ldr, _at(gate), ldg, kind, _at(w_post), _at(w_pre), _at(scale), _ROW_DTYPES[wdtype], alpha, p,
          _at(rng), rstd_z.data_ptr(), rstd_r.data_ptr(), dz.data_ptr(), d, dx.data_ptr(), d, _at(dgate),
