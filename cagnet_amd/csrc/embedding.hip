@@ -498,14 +498,17 @@ __global__ __launch_bounds__(kSortThreads) void emb_small_kernel(KeySource src, 
   if (blockIdx.x > 0) {
     constexpr int V = 16 / (int)sizeof(O);
     const int32_t per_row = (d + V - 1) / V;
-    const int64_t units = src.rows * per_row, step = (int64_t)(gridDim.x - 1) * kSortThreads;
+    const uint32_t step = (gridDim.x - 1) * kSortThreads, first = (blockIdx.x - 1) * kSortThreads + threadIdx.x;
+    const uint32_t rows_on = step / per_row, chunks_on = step % per_row;
     float zero[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) zero[i] = 0.f;
-    for (int64_t u = (int64_t)(blockIdx.x - 1) * kSortThreads + threadIdx.x; u < units; u += step) {
-      const int64_t row = u / per_row;
-      const int32_t j = (int32_t)(u - row * per_row) * V;
+    uint32_t at = first % per_row;
+    for (int64_t row = first / per_row; row < src.rows; row += rows_on) {
+      const int32_t j = (int32_t)at * V;
       store_some<O, V>(out + row * ldo + j, d - j < V ? d - j : V, zero);
+      at += chunks_on;
+      if (at >= (uint32_t)per_row) at -= per_row, ++row;
     }
     return;
   }
