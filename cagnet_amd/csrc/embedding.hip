@@ -67,13 +67,13 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typena
 }
 
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (key, position), digits of up to 9 bits: tables of 2^16 to 2^18 rows take two passes.  A
+// Stable radix sort of (key, position), digits of up to 10 bits: tables of up to a thousand rows take one pass, up to a million two.  A
 // workgroup of 16 wavefronts holds a tile of 4096 keys.  One tile is sorted in LDS by one launch; up to kDirectTiles
 // tiles take two launches a pass (count, scatter: every scatter workgroup adds the tiles' counts up itself, one row of
 // counts a tile); more tiles take a third that scans the counts, one wavefront a digit.
 // ---------------------------------------------------------------------------------------------
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr int kMaxDigit = 9, kMaxRadix = 1 << kMaxDigit;
+constexpr int kMaxDigit = 10, kMaxRadix = 1 << kMaxDigit;
 constexpr int kKeysPerLane = 4;
 constexpr int kSortTile = kSortThreads * kKeysPerLane;
 constexpr int kWaveKeys = kWave * kKeysPerLane;
