@@ -8,123 +8,225 @@
 namespace cg {
 
 // ---------------------------------------------------------------------------------------------
-// Rows of any length: one workgroup per row, the row read again for every pass over it.
+// Rows too long for registers: one workgroup per row, 16 bytes a lane and step, the row read again for every pass over it
+// (it comes from the L2 cache then).
 // ---------------------------------------------------------------------------------------------
+constexpr int kLongThreads = 512;
+
 template <int DT, bool RESIDUAL>
-__global__ __launch_bounds__(kNormThreads) void norm_fwd_rows_kernel(NormArgs a) {
+__global__ __launch_bounds__(kLongThreads) void norm_fwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
+  typedef Span<T, true> C;
+  constexpr int V = C::V;
   __shared__ NormSlots slots;
   int turn = 0;
+  const int32_t step = kLongThreads * V, start = threadIdx.x * V;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
   for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-    const T *z = (const T *)a.z + row * a.ldz;
+    const T *z = (const T *)a.z + row * a.ldz, *x = (const T *)a.x + row * a.ldx, *gate = (const T *)a.gate + row * a.ldgate;
+    C c;
     float s = 0.f;
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) s += (float)z[j] * (float)z[j];
-    const float rho_z = 1.f / sqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
+    for (int32_t j = start; j < a.d; j += step) {
+      float v[V];
+      c.place(j, a.d);
+      c.floats(c.load(z), v);
+      s += c.dot(v, v);
+    }
+    const float rho_z = rsqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_z[row] = rho_z;
     if (!RESIDUAL) {
-      T *h = (T *)a.h + row * a.ldh;
-      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
-        h[j] = rounded<T>((float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j));
+      for (int32_t j = start; j < a.d; j += step) {
+        float v[V], w[V];
+        c.place(j, a.d);
+        c.floats(c.load(z), v);
+        c.weights(a.w_post, a.w_f32, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= rho_z * w[i];
+        c.write((T *)a.h + row * a.ldh, v);
+      }
       continue;
     }
-    const T *x = (const T *)a.x + row * a.ldx;
-    const T *gate = a.gate_kind ? (const T *)a.gate + row * a.ldgate : nullptr;
-    auto sum_at = [&](int32_t j) {
-      float u = (float)z[j] * rho_z * weight_at<T>(a.w_post, a.w_f32, j);
-      if (gate) u *= sigmoid((float)gate[a.gate_kind == CG_GATE_ROW ? 0 : j]);
-      if (a.mask.rng) u = mask_at(key, a.mask, row, j) > 0.f ? u * a.mask.inv_keep : 0.f;
-      return (float)x[j] + a.alpha * weight_at<T>(a.scale, a.w_f32, j) * u;
+    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid((float)gate[0]) : 1.f;
+    auto sum_at = [&](float (&v)[V]) {  // x + u in the columns of c
+      float w[V], t[V];
+      c.floats(c.load(z), v);
+      c.weights(a.w_post, a.w_f32, w);
+      c.weights(a.scale, a.w_f32, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= rho_z * row_sig * (w[i] * (a.alpha * t[i]));
+      if (a.gate_kind == CG_GATE_FULL) {
+        c.floats(c.load(gate), t);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= sigmoid(t[i]);
+      }
+      if (a.mask.rng) c.drop(key, a.mask, row, v);
+      c.floats(c.load(x), t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += t[i];
     };
     s = 0.f;
-    T *r = (T *)a.r + row * a.ldr, *h = (T *)a.h + row * a.ldh;
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
-      const float v = sum_at(j);
-      r[j] = rounded<T>(v);
-      s += v * v;
+    for (int32_t j = start; j < a.d; j += step) {
+      float v[V];
+      c.place(j, a.d);
+      sum_at(v);
+      s += c.dot(v, v);
+      c.write((T *)a.r + row * a.ldr, v);
     }
-    const float rho_r = 1.f / sqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
+    const float rho_r = rsqrtf(row_sum<kWave, true>(s, slots, turn) / (float)a.d + a.eps);
     if (threadIdx.x == 0) a.rstd_r[row] = rho_r;
-    // h comes from the sum before its rounding to the stored type
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) h[j] = rounded<T>(sum_at(j) * rho_r * weight_at<T>(a.w_pre, a.w_f32, j));
+    for (int32_t j = start; j < a.d; j += step) {  // h comes from the sum before its rounding to the stored type
+      float v[V], w[V];
+      c.place(j, a.d);
+      sum_at(v);
+      c.weights(a.w_pre, a.w_f32, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= rho_r * w[i];
+      c.write((T *)a.h + row * a.ldh, v);
+    }
   }
 }
 
 // The gradients of the weights are sums over rows: every workgroup adds its rows up in its own slice of `partial`
 // (each column belongs to one thread), and a second kernel adds the slices in order.
 template <int DT, bool RESIDUAL>
-__global__ __launch_bounds__(kNormThreads) void norm_bwd_rows_kernel(NormArgs a) {
+__global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
+  typedef Span<T, true> C;
+  constexpr int V = C::V;
   __shared__ NormSlots slots;
   int turn = 0;
+  const int32_t step = kLongThreads * V, start = threadIdx.x * V;
   MaskKey key = {0, 0, 0, 0};
   if (RESIDUAL && a.mask.rng) key = mask_key(a.mask.rng);
-  float *q = a.partial + (int64_t)blockIdx.x * (RESIDUAL ? 2 : 1) * a.d, *dwp = q + a.d;
-  for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
-    q[j] = 0.f;
-    if (RESIDUAL) dwp[j] = 0.f;
-  }
-  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-    const T *z = (const T *)a.z + row * a.ldz;
-    const T *dh = a.dh ? (const T *)a.dh + row * a.lddh : nullptr;
+  float *q = a.partial + (int64_t)blockIdx.x * (RESIDUAL ? 2 : 1) * a.d, *p = q + a.d;
+  C c;
+  bool first = true;
+  auto add_to = [&](float *sums, const float (&v)[V]) {  // the workgroup's first row writes
+    float old[V];
+    if (c.dup == 0 && a.d >= V) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) old[i] = 0.f;
+      if (!first) load_pack<float, V>(sums + c.at, old);
+#pragma unroll
+      for (int i = 0; i < V; ++i) old[i] += v[i];
+      store_pack<float, V>(sums + c.at, old);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) old[i] = !first && c.counts(i) ? sums[c.at + i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (c.counts(i)) sums[c.at + i] = old[i] + v[i];
+  };
+  for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x, first = false) {
+    const T *z = (const T *)a.z + row * a.ldz, *dh = (const T *)a.dh + row * a.lddh, *r = (const T *)a.r_in + row * a.ldr_in;
+    const T *dr = (const T *)a.dr + row * a.lddr, *gate = (const T *)a.gate + row * a.ldgate;
     T *dz = (T *)a.dz + row * a.lddz;
-    const float rho_z = a.rstd_z[row];
-    if (!RESIDUAL) {
+    const float rho_z = a.rstd_z[row], rho_r = RESIDUAL ? a.rstd_r[row] : 0.f;
+    const T *g = dh, *unit = RESIDUAL ? r : z;  // the norm whose output's gradient is given
+    const void *weight = RESIDUAL ? a.w_pre : a.w_post;
+    const float rho = RESIDUAL ? rho_r : rho_z;
+    float mean = 0.f;
+    if (a.dh) {
       float s = 0.f;
-      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
-        s += (float)dh[j] * weight_at<T>(a.w_post, a.w_f32, j) * ((float)z[j] * rho_z);
-      const float m = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
-      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
-        const float zh = (float)z[j] * rho_z, g = (float)dh[j];
-        q[j] += g * zh;
-        dz[j] = rounded<T>(rho_z * (g * weight_at<T>(a.w_post, a.w_f32, j) - zh * m));
+      for (int32_t j = start; j < a.d; j += step) {
+        float t[V], h[V], w[V];
+        c.place(j, a.d);
+        c.floats(c.load(g), t);
+        c.floats(c.load(unit), h);
+        c.weights(weight, a.w_f32, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          h[i] *= rho;
+          w[i] *= t[i];
+          t[i] *= h[i];
+        }
+        add_to(RESIDUAL ? p : q, t);
+        s += c.dot(w, h);
+      }
+      mean = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
+    }
+    auto into = [&](float (&v)[V]) {  // gradient of that norm's input, of the residual sum with dr
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = 0.f;
+      if (a.dh) {
+        float h[V], w[V];
+        c.floats(c.load(g), v);
+        c.floats(c.load(unit), h);
+        c.weights(weight, a.w_f32, w);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = rho * (v[i] * w[i] - h[i] * rho * mean);
+      }
+      if (RESIDUAL && a.dr) {
+        float t[V];
+        c.floats(c.load(dr), t);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] += t[i];
+      }
+    };
+    if (!RESIDUAL) {
+      for (int32_t j = start; j < a.d; j += step) {
+        float v[V];
+        c.place(j, a.d);
+        into(v);
+        c.write(dz, v);
       }
       continue;
     }
-    const T *r = (const T *)a.r_in + row * a.ldr_in;
-    const T *dr = a.dr ? (const T *)a.dr + row * a.lddr : nullptr;
-    const T *gate = a.gate_kind ? (const T *)a.gate + row * a.ldgate : nullptr;
-    const float rho_r = a.rstd_r[row];
-    float mean_r = 0.f;
-    if (dh) {
-      float s = 0.f;
-      for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads)
-        s += (float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) * ((float)r[j] * rho_r);
-      mean_r = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
-    }
-    auto into = [&](int32_t j) {  // gradient of the residual sum
-      float v = dr ? (float)dr[j] : 0.f;
-      if (dh) v += rho_r * ((float)dh[j] * weight_at<T>(a.w_pre, a.w_f32, j) - (float)r[j] * rho_r * mean_r);
-      return v;
+    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid((float)gate[0]) : 1.f;
+    auto through = [&](float (&D)[V], float (&zh)[V], float (&f)[V], bool outputs) {  // f: gradient of the normalised z
+      float w[V], t[V], sig[V];
+      into(D);
+      if (outputs) c.write((T *)a.dx + row * a.lddx, D);
+      if (a.mask.rng) c.drop(key, a.mask, row, D);
+      c.floats(c.load(z), zh);
+      c.weights(a.w_post, a.w_f32, w);
+      c.weights(a.scale, a.w_f32, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        zh[i] *= rho_z;
+        f[i] = D[i] * (w[i] * (a.alpha * t[i]));
+        sig[i] = row_sig;
+      }
+      if (a.gate_kind == CG_GATE_FULL) {
+        c.floats(c.load(gate), t);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          sig[i] = sigmoid(t[i]);
+          t[i] = f[i] * zh[i] * (sig[i] * (1.f - sig[i]));
+        }
+        if (outputs) c.write((T *)a.dgate + row * a.lddgate, t);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        D[i] *= sig[i] * zh[i];
+        f[i] *= a.gate_kind == CG_GATE_FULL ? sig[i] : 1.f;
+      }
     };
-    auto gate_at = [&](int32_t j) { return gate ? sigmoid((float)gate[a.gate_kind == CG_GATE_ROW ? 0 : j]) : 1.f; };
-    auto keep_at = [&](int32_t j) { return a.mask.rng ? mask_at(key, a.mask, row, j) : 1.f; };
-    float s = 0.f, sg = 0.f;
-    T *dx = (T *)a.dx + row * a.lddx;
-    T *dgate = a.dgate ? (T *)a.dgate + row * a.lddgate : nullptr;
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
-      const float D = into(j), zh = (float)z[j] * rho_z, sig = gate_at(j), Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
-      const float e = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j);
-      dx[j] = rounded<T>(D);
-      s += e * sig * zh;
-      q[j] += Dm * sig * zh;
-      if (dh) dwp[j] += (float)dh[j] * ((float)r[j] * rho_r);
-      const float dg = e * zh * (sig * (1.f - sig));
-      if (a.gate_kind == CG_GATE_ROW)
-        sg += dg;
-      else if (dgate)
-        dgate[j] = rounded<T>(dg);
+    float s = 0.f;
+    for (int32_t j = start; j < a.d; j += step) {
+      float D[V], zh[V], f[V];
+      c.place(j, a.d);
+      through(D, zh, f, true);
+      add_to(q, D);
+      if (!a.dh && first) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (c.counts(i)) p[c.at + i] = 0.f;
+      }
+      s += c.dot(f, zh);
     }
-    const float mean_z = row_sum<kWave, true>(s, slots, turn) / (float)a.d;
-    if (a.gate_kind == CG_GATE_ROW) {
-      sg = row_sum<kWave, true>(sg, slots, turn);
-      if (dgate && threadIdx.x == 0) dgate[0] = rounded<T>(sg);
-    }
-    for (int32_t j = threadIdx.x; j < a.d; j += kNormThreads) {
-      const float D = into(j), zh = (float)z[j] * rho_z, Dm = keep_at(j) > 0.f ? D * keep_at(j) : 0.f;
-      const float f = Dm * a.alpha * weight_at<T>(a.scale, a.w_f32, j) * weight_at<T>(a.w_post, a.w_f32, j) * gate_at(j);
-      dz[j] = rounded<T>(rho_z * (f - zh * mean_z));
+    s = row_sum<kWave, true>(s, slots, turn);
+    if (a.gate_kind == CG_GATE_ROW && threadIdx.x == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));
+    const float mean_z = s / (float)a.d;
+    for (int32_t j = start; j < a.d; j += step) {
+      float D[V], zh[V], f[V];
+      c.place(j, a.d);
+      through(D, zh, f, false);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = rho_z * row_sig * (f[i] - zh[i] * mean_z);
+      c.write(dz, f);
     }
   }
 }
@@ -201,7 +303,7 @@ template <bool RESIDUAL>
 static int norm_fwd(const NormArgs &a, int dtype, hipStream_t s) {
   if (norm_shape(a.d, dtype, false).lanes > 0) return launch_norm_fwd(a, RESIDUAL, dtype, s);
   const int64_t groups = a.n < 256 * 32 ? a.n : 256 * 32;
-#define CG_CALL(DT) norm_fwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
+#define CG_CALL(DT) norm_fwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kLongThreads, 0, s>>>(a)
   CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();
@@ -214,7 +316,7 @@ static int norm_bwd(const NormArgs &a, int dtype, void *dw_post, void *dw_pre, v
   if (groups > 0 && norm_shape(a.d, dtype, RESIDUAL).lanes > 0) {
     CG_TRY(launch_norm_bwd(a, RESIDUAL, dtype, groups, s));
   } else if (groups > 0) {
-#define CG_CALL(DT) norm_bwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kNormThreads, 0, s>>>(a)
+#define CG_CALL(DT) norm_bwd_rows_kernel<DT, RESIDUAL><<<(unsigned)groups, kLongThreads, 0, s>>>(a)
     CG_BY_DTYPE(dtype, CG_CALL)
 #undef CG_CALL
     CG_LAUNCH_CHECK();

@@ -16,7 +16,7 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i < c[k].live) dst[((int)threadIdx.x + k * (int)blockDim.x) * V + i] = acc[k][i];
+        if (c[k].counts(i)) dst[c[k].at + i] = acc[k][i];
     return;
   }
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
@@ -26,7 +26,7 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)
     for (int i = 0; i < V; ++i) {
 #pragma unroll
       for (int off = LANES; off < kWave; off <<= 1) acc[k][i] += __shfl_xor(acc[k][i], off, kWave);
-      if (lane < LANES) lds[wave * (LANES * K * V) + (lane + k * LANES) * V + i] = acc[k][i];
+      if (lane < LANES && c[k].counts(i)) lds[wave * (LANES * K * V) + c[k].at + i] = acc[k][i];
     }
   __syncthreads();
   for (int j = threadIdx.x; j < d; j += kNormThreads) {
@@ -38,27 +38,33 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)
   __syncthreads();
 }
 
+// The bound on registers: four wavefronts a SIMD where 8 elements of 16 bits a lane miss that by a few (without it
+// 2,343,750 x 64 bf16 takes 420 us instead of 353).
 template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
-__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void norm_bwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, RESIDUAL && DT != CG_F32 && K == 1 ? 4 : 1) void norm_bwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T, RAGGED> C;
+  typedef Span<T, RAGGED> C;
   constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
   __shared__ NormSlots slots;
   __shared__ float lds[WHOLE ? 1 : kNormWaves * LANES * K * V];
   int turn = 0;
-  const int lane = WHOLE ? threadIdx.x : threadIdx.x % LANES, team = WHOLE ? 0 : threadIdx.x / LANES;
+  // Where a wavefront holds one row its number is made uniform, which moves the row's addresses to the scalar unit:
+  // 250,000 x 300 float32 with row gates and dropout 432 -> 365 us.  With 16 elements a lane the scalar registers run
+  // out and it costs instead (249,169 x 602 bf16: 417 -> 457 us).
+  constexpr bool UNIFORM = !WHOLE && LANES == kWave && K * V < 16;
+  const int lane = WHOLE ? threadIdx.x : threadIdx.x % LANES;
+  const int team = WHOLE ? 0 : UNIFORM ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : threadIdx.x / LANES;
   const int lanes = WHOLE ? blockDim.x : LANES;
   C c[K];
   float wz[K][V], wr[K][V], q[K][V], p[K][V];  // alpha scale w_post (w_post alone for rms_norm), w_pre, column sums
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int32_t j = (lane + k * lanes) * V;
-    c[k].place(j, a.d);
-    weight_chunk<T, V>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
+    c[k].place((lane + k * lanes) * V, a.d);
+    c[k].weights(a.w_post, a.w_f32, wz[k]);
     if (RESIDUAL) {
       float s[V];
-      weight_chunk<T, V>(a.scale, a.w_f32, j, c[k].live, s);
-      weight_chunk<T, V>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
+      c[k].weights(a.scale, a.w_f32, s);
+      c[k].weights(a.w_pre, a.w_f32, wr[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) wz[k][i] *= a.alpha * s[i];
     }
@@ -89,8 +95,8 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
           zh[k][i] *= rho_z;
           q[k][i] += t[k][i] * zh[k][i];
           t[k][i] *= wz[k][i];
-          s += t[k][i] * zh[k][i];
         }
+        s += c[k].dot(t[k], zh[k]);
       }
       const float m = row_sum<LANES, WHOLE>(s, slots, turn) * inv_d;
 #pragma unroll
@@ -129,8 +135,8 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
           rh[k][i] *= rho_r;
           p[k][i] += D[k][i] * rh[k][i];
           D[k][i] *= wr[k][i];
-          s += D[k][i] * rh[k][i];
         }
+        s += c[k].dot(D[k], rh[k]);
       }
       const float m = row_sum<LANES, WHOLE>(s, slots, turn) * inv_d;
 #pragma unroll
@@ -159,7 +165,7 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
       c[k].write((T *)a.dx + row * a.lddx, D[k]);
       c[k].floats(rz[k], zh[k]);
       if (a.mask.rng)
-        drop_chunk<V>(key, a.mask, row, (lane + k * lanes) * V, D[k]);
+        c[k].drop(key, a.mask, row, D[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) zh[k][i] *= rho_z;
       if (a.gate_kind == CG_GATE_FULL) {
@@ -180,8 +186,7 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
           D[k][i] *= wz[k][i];
         }
       }
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += D[k][i] * zh[k][i];
+      s += c[k].dot(D[k], zh[k]);
     }
     s = row_sum<LANES, WHOLE>(s, slots, turn);
     if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));

@@ -5,10 +5,12 @@
 
 namespace cg {
 
+// 128 registers or fewer let four wavefronts run on a SIMD, 168 three: the bounds hold the compiler to what it misses by
+// a few registers otherwise.
 template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
-__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void norm_fwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, !RESIDUAL ? 1 : DT != CG_F32 && K == 2 ? 4 : 3) void norm_fwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T, RAGGED> C;
+  typedef Span<T, RAGGED> C;
   constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
   __shared__ NormSlots slots;
   int turn = 0;
@@ -18,13 +20,12 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
   float wz[K][V], wr[K][V];  // alpha scale w_post (w_post alone for rms_norm) and w_pre
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int32_t j = (lane + k * lanes) * V;
-    c[k].place(j, a.d);
-    weight_chunk<T, V>(a.w_post, a.w_f32, j, c[k].live, wz[k]);
+    c[k].place((lane + k * lanes) * V, a.d);
+    c[k].weights(a.w_post, a.w_f32, wz[k]);
     if (RESIDUAL) {
       float s[V];
-      weight_chunk<T, V>(a.scale, a.w_f32, j, c[k].live, s);
-      weight_chunk<T, V>(a.w_pre, a.w_f32, j, c[k].live, wr[k]);
+      c[k].weights(a.scale, a.w_f32, s);
+      c[k].weights(a.w_pre, a.w_f32, wr[k]);
 #pragma unroll
       for (int i = 0; i < V; ++i) wz[k][i] *= a.alpha * s[i];
     }
@@ -52,8 +53,7 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       c[k].floats(rz[k], v[k]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s += v[k][i] * v[k][i];
+      s += c[k].dot(v[k], v[k]);
     }
     const float rho_z = rsqrtf(row_sum<LANES, WHOLE>(s, slots, turn) * inv_d + a.eps);
     if (lane == 0) a.rstd_z[row] = rho_z;
@@ -80,13 +80,11 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads) void 
         for (int i = 0; i < V; ++i) v[k][i] *= sigmoid(g[i]);
       }
       if (a.mask.rng)
-        drop_chunk<V>(key, a.mask, row, (lane + k * lanes) * V, v[k]);
+        c[k].drop(key, a.mask, row, v[k]);
       c[k].floats(rx[k], x);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        v[k][i] += x[i];
-        s += v[k][i] * v[k][i];
-      }
+      for (int i = 0; i < V; ++i) v[k][i] += x[i];
+      s += c[k].dot(v[k], v[k]);
       c[k].write((T *)a.r + row * a.ldr, v[k]);
     }
     const float rho_r = rsqrtf(row_sum<LANES, WHOLE>(s, slots, turn) * inv_d + a.eps);

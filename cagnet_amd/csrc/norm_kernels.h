@@ -50,7 +50,7 @@ static inline NormShape norm_shape(int32_t d, int dtype, bool residual_bwd) {
     const int64_t waves = ceil_div64(c, (int64_t)kWave * chunks);
     if (waves <= kNormMaxWaves) return NormShape{kWave, chunks, (int)waves * kWave, true};
   }
-  return NormShape{0, 0, kNormThreads, true};
+  return NormShape{0, 0, 512, true};
 }
 static inline int norm_rows_at_once(const NormShape &s) { return s.whole ? 1 : s.threads / s.lanes; }
 
@@ -64,8 +64,7 @@ typedef float NormSlots[2][kNormMaxWaves];
 
 template <int LANES, bool WHOLE>
 __device__ __forceinline__ float row_sum(float v, NormSlots &slots, int &turn) {
-#pragma unroll
-  for (int off = LANES / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  v = team_sum_of<LANES>(v);
   if (!WHOLE) return v;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   if (lane == 0) slots[turn][wave] = v;
@@ -83,11 +82,87 @@ __device__ __forceinline__ float sigmoid(float a) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504f));
 }
 
-// a weight vector's elements of one chunk, ones for a null pointer, zeros behind the row's end
-template <typename T, int V>
-__device__ __forceinline__ void weight_chunk(const void *w, int w_f32, int32_t j, int live, float (&out)[V]) {
+// ---------------------------------------------------------------------------------------------
+// A lane's 16 bytes of a row.  Where the row ends inside them, or before them, the lane takes the row's last 16 bytes
+// instead: the elements it repeats from the lane before (the first `dup`) are computed again, to the same bits, but
+// count in no sum.  So every load and store is whole and none needs shifting into place.  RAGGED: rows whose length is
+// not a whole number of chunks; otherwise a lane's elements count all or none (dup 0 or V).  Rows shorter than 16 bytes
+// are moved element by element.
+// ---------------------------------------------------------------------------------------------
+template <typename T, bool RAGGED>
+struct Span {
+  static constexpr int V = 16 / (int)sizeof(T);
+  typedef typename Pack<T, V>::type vec;
+
+  int32_t at, dup, d;
+
+  __device__ __forceinline__ void place(int32_t j, int32_t d_) {
+    d = d_;
+    at = j < d - V ? j : (d > V ? d - V : 0);
+    dup = j - at < V ? j - at : V;
+  }
+  __device__ __forceinline__ bool any() const { return dup < V; }
+  // element i of the lane counts
+  __device__ __forceinline__ bool counts(int i) const { return RAGGED ? i >= dup && i < d : dup == 0; }
+  __device__ __forceinline__ Raw load(const T *row) const {
+    if (!RAGGED || d >= V) return __builtin_bit_cast(Raw, *reinterpret_cast<const vec *>(row + at));
+    vec q = {};
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = i < live ? weight_at<T>(w, w_f32, j + i) : 0.f;
-}
+    for (int i = 0; i < V; ++i) q[i] = row[i < d ? i : d - 1];
+    return __builtin_bit_cast(Raw, q);
+  }
+  __device__ __forceinline__ void floats(Raw r, float (&out)[V]) const {
+    const vec q = __builtin_bit_cast(vec, r);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = (float)q[i];
+  }
+  __device__ __forceinline__ void write(T *row, const float (&in)[V]) const {
+    vec q = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) q[i] = rounded<T>(in[i]);
+    if (!any()) return;
+    if (!RAGGED || d >= V) {
+      *reinterpret_cast<vec *>(row + at) = q;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i)
+        if (i < d) row[i] = q[i];
+    }
+  }
+  // sum of a * b over the elements that count
+  __device__ __forceinline__ float dot(const float (&a)[V], const float (&b)[V]) const {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += !RAGGED || counts(i) ? a[i] * b[i] : 0.f;
+    return RAGGED || dup == 0 ? s : 0.f;
+  }
+  // a weight vector's elements, ones for a null pointer
+  __device__ __forceinline__ void weights(const void *w, int w_f32, float (&out)[V]) const {
+    if (!w) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = 1.f;
+    } else if (RAGGED && d < V) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = weight_at<T>(w, w_f32, i < d ? i : d - 1);
+    } else if (w_f32) {
+      load_pack<float, V>(static_cast<const float *>(w) + at, out);
+    } else {
+      load_pack<T, V>(static_cast<const T *>(w) + at, out);
+    }
+  }
+  // v / (1 - p) for kept elements, 0 for dropped ones.  The generator decides aligned groups of four columns; where the
+  // lane's columns are not aligned, the decisions of its own V columns and of the V before are shifted together.
+  __device__ __forceinline__ void drop(const MaskKey &key, const Mask &m, int64_t row, float (&v)[V]) const {
+    if (!RAGGED) {
+      drop_chunk<V>(key, m, row, at, v);
+      return;
+    }
+    const int32_t j = at + dup;  // the aligned columns the lane would have without the row's end (dup < V)
+    uint32_t bits = keep_bits<V>(key, m, row, j);
+    if (dup > 0 && dup < V) bits = ((bits << V) | keep_bits<V>(key, m, row, j - V)) >> (V - dup);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (bits >> i) & 1u ? v[i] * m.inv_keep : 0.f;
+  }
+};
 
 }  // namespace cg

@@ -141,6 +141,28 @@ struct Chunk {
   }
 };
 
+// Sum over teams of LANES consecutive lanes of a wavefront, the same bits in every lane, without a trip through LDS: data
+// parallel primitives inside 16 lanes (swap in pairs, in quads, mirror 8, mirror 16: sums of equal groups, so a mirror
+// does what an exclusive-or of the lane number would), then the exchanges of halves between rows of 16 and of 32.
+template <int LANES>
+__device__ __forceinline__ float team_sum_of(float v) {
+#define CG_DPP(ctrl) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, true))
+  if (LANES >= 2) v += CG_DPP(0xB1);
+  if (LANES >= 4) v += CG_DPP(0x4E);
+  if (LANES >= 8) v += CG_DPP(0x141);
+  if (LANES >= 16) v += CG_DPP(0x140);
+#undef CG_DPP
+  if (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  if (LANES >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  return v;
+}
+
 // A weight vector: float32, or the type of the activations; a null pointer stands for ones.
 template <typename T>
 __device__ __forceinline__ float weight_at(const void *w, int w_f32, int32_t j) {
@@ -220,6 +242,20 @@ __device__ __forceinline__ float mask_at(const MaskKey &k, const Mask &m, int64_
   mask_words(k, (uint32_t)row, (uint32_t)j >> 2, w);
   const uint32_t mine = (j & 2) ? ((j & 1) ? w[3] : w[2]) : ((j & 1) ? w[1] : w[0]);
   return mine > m.last ? m.inv_keep : 0.f;
+}
+
+// bit i: the element in column j + i is kept (j a multiple of four)
+template <int V>
+__device__ __forceinline__ uint32_t keep_bits(const MaskKey &k, const Mask &m, int64_t row, int32_t j) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int b = 0; b < V / 4; ++b) {
+    uint32_t w[4];
+    mask_words(k, (uint32_t)row, (uint32_t)(j / 4 + b), w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= w[i] > m.last ? 1u << (4 * b + i) : 0u;
+  }
+  return bits;
 }
 
 // v / (1 - p) for the kept elements of the chunk that starts at column j (a multiple of four), 0 for the others
