@@ -1,6 +1,6 @@
 // Forward pass of rms_norm and norm_residual with the row in registers: every operand is read once and every result
 // written once, the statistics come from the registers in between.  Lanes and chunks per row: norm_shape.  The waves
-// loop over rows (all of them side by side through memory) and keep their columns' weights in registers.
+// loop over rows, all of them side by side through memory, with their columns' weights in registers.
 #include "norm_kernels.h"
 
 namespace cg {
@@ -118,7 +118,13 @@ template <int DT>
 static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
   constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
   const NormShape sh = norm_shape(a.d, DT, false);
-  const int64_t want = ceil_div64(a.n, norm_rows_at_once(sh)), most = sh.whole ? 256 * 16 / (sh.threads / kWave) : 256 * 8;
+  // Few rows a wave: the loads of a wave's next row would wait for the stores of the row before (they are counted
+  // together and in order), those of a new wave do not.  124,584 x 602 float32: 242 us with 8 workgroups per compute unit
+  // in all, 228 with 32, 210 with 128.  Partial chunks of 16-bit elements pay more per wave for their weights and
+  // addresses: 249,169 x 602 bf16 with dropout 328 us with 8 or 32, 397 with 128.
+  const bool costly = residual && DT != CG_F32 && !sh.whole && a.d % 8 != 0;
+  const int64_t want = ceil_div64(a.n, norm_rows_at_once(sh));
+  const int64_t most = sh.whole ? 256 * 256 / (sh.threads / kWave) : costly ? 256 * 32 : 256 * 128;
   groups = want < most ? want : most;
   if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);
   if (sh.lanes == 4) return go<DT, 4, 1, false>(a, residual, sh, groups, s);

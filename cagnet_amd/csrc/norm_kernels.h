@@ -116,10 +116,14 @@ struct Span {
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = (float)q[i];
   }
-  __device__ __forceinline__ void write(T *row, const float (&in)[V]) const {
+  __device__ __forceinline__ Raw packed(const float (&in)[V]) const {
     vec q = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) q[i] = rounded<T>(in[i]);
+    return __builtin_bit_cast(Raw, q);
+  }
+  __device__ __forceinline__ void put(T *row, Raw r) const {
+    const vec q = __builtin_bit_cast(vec, r);
     if (!any()) return;
     if (!RAGGED || d >= V) {
       *reinterpret_cast<vec *>(row + at) = q;
@@ -129,6 +133,7 @@ struct Span {
         if (i < d) row[i] = q[i];
     }
   }
+  __device__ __forceinline__ void write(T *row, const float (&in)[V]) const { put(row, packed(in)); }
   // sum of a * b over the elements that count
   __device__ __forceinline__ float dot(const float (&a)[V], const float (&b)[V]) const {
     float s = 0.f;

@@ -421,16 +421,18 @@ class Embedding(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, idx, scale):
-        flat = idx.reshape(-1)
+        flat = idx if idx.dim() == 1 else idx.reshape(-1)
         ctx.save_for_backward(flat)
         ctx.rows, ctx.width, ctx.scale = table.shape[0], table.shape[1], scale
-        return ops.embedding_fwd(table, flat, scale).view(*idx.shape, table.shape[1])
+        out = ops.embedding_fwd(table, flat, scale)
+        return out if idx.dim() == 1 else out.view(*idx.shape, table.shape[1])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         (flat,) = ctx.saved_tensors
-        return ops.embedding_bwd(g.reshape(-1, ctx.width), flat, ctx.rows, ctx.scale), None, None
+        g = g if g.dim() == 2 else g.reshape(-1, ctx.width)
+        return ops.embedding_bwd(g, flat, ctx.rows, ctx.scale), None, None
 
 
 def embedding(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
