@@ -16,7 +16,7 @@ constexpr int kLongThreads = 512;
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kLongThreads) void norm_fwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Span<T, true> C;
+  typedef Span<T, kPartChunk> C;
   constexpr int V = C::V;
   __shared__ NormSlots slots;
   int turn = 0;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_fwd_rows_kernel(NormArgs a)
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Span<T, true> C;
+  typedef Span<T, kPartChunk> C;
   constexpr int V = C::V;
   __shared__ NormSlots slots;
   int turn = 0;
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
   bool first = true;
   auto add_to = [&](float *sums, const float (&v)[V]) {  // the workgroup's first row writes
     float old[V];
-    if (c.dup == 0 && a.d >= V) {
+    if (c.dup == 0) {
 #pragma unroll
       for (int i = 0; i < V; ++i) old[i] = 0.f;
       if (!first) load_pack<float, V>(sums + c.at, old);

@@ -38,12 +38,14 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)
   __syncthreads();
 }
 
-// The bound on registers: four wavefronts a SIMD where 8 elements of 16 bits a lane miss that by a few (without it
-// 2,343,750 x 64 bf16 takes 420 us instead of 353).
-template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
-__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, RESIDUAL && DT != CG_F32 && K == 1 ? 4 : 1) void norm_bwd_kernel(NormArgs a) {
+// The bound on registers, where 8 elements of 16 bits a lane miss it by a few: four wavefronts a SIMD for rows of whole
+// chunks (2,343,750 x 64 bf16: 420 us without, 353 with), three for others, which would have to spill for the fourth
+// (3,658,536 x 41 bf16 with row gates and dropout: 872 us with four, 705 with three).
+template <int DT, int LANES, int K, bool WHOLE, int FIT, bool RESIDUAL>
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads,
+                             !RESIDUAL || DT == CG_F32 || K > 1 ? 1 : FIT == kPartChunk ? 3 : 4) void norm_bwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Span<T, RAGGED> C;
+  typedef Span<T, FIT> C;
   constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
   __shared__ NormSlots slots;
   __shared__ float lds[WHOLE ? 1 : kNormWaves * LANES * K * V];
@@ -203,20 +205,22 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, RESID
   if (RESIDUAL) fold_columns<C, LANES, K, WHOLE>(p, c, lds, slice + a.d, a.d);
 }
 
-template <int DT, int LANES, int K, bool WHOLE, bool RAGGED>
-static int go_ragged(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
+template <int DT, int LANES, int K, bool WHOLE, int FIT>
+static int go_fit(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
   if (residual)
-    norm_bwd_kernel<DT, LANES, K, WHOLE, RAGGED, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
+    norm_bwd_kernel<DT, LANES, K, WHOLE, FIT, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   else
-    norm_bwd_kernel<DT, LANES, K, WHOLE, RAGGED, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
+    norm_bwd_kernel<DT, LANES, K, WHOLE, FIT, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   CG_LAUNCH_CHECK();
   return CG_OK;
 }
 
 template <int DT, int LANES, int K, bool WHOLE>
 static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
-  if (a.d % (DT == CG_F32 ? 4 : 8) == 0) return go_ragged<DT, LANES, K, WHOLE, false>(a, residual, sh, groups, s);
-  return go_ragged<DT, LANES, K, WHOLE, true>(a, residual, sh, groups, s);
+  constexpr int V = DT == CG_F32 ? 4 : 8;
+  if (a.d % V == 0) return go_fit<DT, LANES, K, WHOLE, kWholeChunks>(a, residual, sh, groups, s);
+  if (LANES == 4 && a.d < V) return go_fit<DT, 4, 1, false, kShortRow>(a, residual, sh, groups, s);
+  return go_fit<DT, LANES, K, WHOLE, kPartChunk>(a, residual, sh, groups, s);
 }
 
 template <int DT>

@@ -7,10 +7,10 @@ namespace cg {
 
 // 128 registers or fewer let four wavefronts run on a SIMD, 168 three: the bounds hold the compiler to what it misses by
 // a few registers otherwise.
-template <int DT, int LANES, int K, bool WHOLE, bool RAGGED, bool RESIDUAL>
-__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, !RESIDUAL ? 1 : DT != CG_F32 && K == 2 ? 4 : 3) void norm_fwd_kernel(NormArgs a) {
+template <int DT, int LANES, int K, bool WHOLE, int FIT, bool RESIDUAL>
+__global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, !RESIDUAL ? 1 : (DT != CG_F32 && K == 2) || K == 3 ? 4 : 3) void norm_fwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
-  typedef Span<T, RAGGED> C;
+  typedef Span<T, FIT> C;
   constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
   __shared__ NormSlots slots;
   int turn = 0;
@@ -98,20 +98,22 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads, !RESI
   }
 }
 
-template <int DT, int LANES, int K, bool WHOLE, bool RAGGED>
-static int go_ragged(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
+template <int DT, int LANES, int K, bool WHOLE, int FIT>
+static int go_fit(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
   if (residual)
-    norm_fwd_kernel<DT, LANES, K, WHOLE, RAGGED, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
+    norm_fwd_kernel<DT, LANES, K, WHOLE, FIT, true><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   else
-    norm_fwd_kernel<DT, LANES, K, WHOLE, RAGGED, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
+    norm_fwd_kernel<DT, LANES, K, WHOLE, FIT, false><<<(unsigned)groups, sh.threads, 0, s>>>(a);
   CG_LAUNCH_CHECK();
   return CG_OK;
 }
 
 template <int DT, int LANES, int K, bool WHOLE>
 static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t groups, hipStream_t s) {
-  if (a.d % (DT == CG_F32 ? 4 : 8) == 0) return go_ragged<DT, LANES, K, WHOLE, false>(a, residual, sh, groups, s);
-  return go_ragged<DT, LANES, K, WHOLE, true>(a, residual, sh, groups, s);
+  constexpr int V = DT == CG_F32 ? 4 : 8;
+  if (a.d % V == 0) return go_fit<DT, LANES, K, WHOLE, kWholeChunks>(a, residual, sh, groups, s);
+  if (LANES == 4 && a.d < V) return go_fit<DT, 4, 1, false, kShortRow>(a, residual, sh, groups, s);
+  return go_fit<DT, LANES, K, WHOLE, kPartChunk>(a, residual, sh, groups, s);
 }
 
 template <int DT>
