@@ -135,6 +135,8 @@ def test_dropout_beyond_32_bit_offsets(cuda):
 EMBED = [  # n, rows, d, pad
     (1, 1, 1, 0), (1, 3, 5, 0), (7, 2, 16, 0), (64, 1000, 4, 0), (300, 50, 41, 0), (5000, 17, 128, 0), (2048, 600, 602, 1),
     (2049, 70000, 8, 0), (9000, 300000, 3, 0), (4097, 1, 33, 0), (20000, 40, 257, 2), (31, 9, 4099, 0), (6000, 513, 64, 0),
+    # one tile, two tiles and more tiles of indices than the scatter adds up itself; tables of one, two and three sort passes
+    (4096, 1023, 2, 0), (4097, 1024, 2, 0), (300_000, 1000, 3, 0), (5000, (1 << 20) + 5, 2, 0),
 ]
 
 
@@ -227,7 +229,9 @@ def test_embedding_beyond_32_bit_offsets(cuda):
 # ---------------------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 1, 0), (1, 2, 0), (5, 3, 0), (2, 16, 0), (700, 16, 0), (33, 41, 0), (260, 128, 0), (9, 255, 0), (40, 256, 0), (17, 260, 1),
           (50, 602, 0), (12, 1024, 0), (3, 1025, 3), (6, 2048, 0), (5, 2563, 0), (4, 4096, 0), (3, 8200, 1), (2, 16384, 0), (2, 20011, 0),
-          (2500, 24, 0), (1, 602, 0)]
+          (2500, 24, 0), (1, 602, 0),
+          # several steps of every team: more rows than the workgroups of a launch hold at once, and the longest rows of each kind
+          (70_000, 8, 0), (4200, 300, 0), (700, 1030, 0), (3, 5003, 1), (2, 8192, 0), (600, 8201, 0)]
 
 
 def wtypes(t):
@@ -368,6 +372,24 @@ def test_norm_gate_extremes(cuda):
     assert not bool(r[0].any()) and not bool(r[2].any()) and bool(r[1].all()) and bool(r[3].all())
     out = ops.norm_residual_bwd(z, None, z, r, None, None, rz, rr, gate)
     assert out[2].flatten().tolist() == [0.0] * 4 and all(bool(torch.isfinite(v).all()) for v in out[:2])
+
+
+def test_dropped_elements_of_a_broken_block_leave_the_residual(cuda):
+    """A block output with NaN: its dropped elements add nothing, in both directions."""
+    from cagnet_amd import ops
+
+    z = torch.randn(6, 50, generator=torch.Generator().manual_seed(1))
+    z[2, 7] = float("nan")
+    x = torch.randn(6, 50, generator=torch.Generator().manual_seed(2))
+    keep = ref.keep_mask(3, 9, 6, 50, 0.5)
+    rng = ops.rng_state(3, cuda, 9)
+    r, _, rz, rr = ops.norm_residual_fwd(z.to(cuda), x.to(cuda), None, None, p=0.5, rng=rng)
+    assert torch.equal(r.cpu()[~keep], x[~keep]) and bool(torch.isnan(r.cpu()[2][keep[2]]).all())
+    assert bool(torch.isfinite(r[[0, 1, 3, 4, 5]]).all())
+    dr = torch.full((6, 50), float("inf"))
+    dr[keep] = 1.0
+    out = ops.norm_residual_bwd(dr.to(cuda), None, z.to(cuda), r, None, None, rz, rr, p=0.5, rng=rng)
+    assert bool(torch.isfinite(out[0][[0, 1, 3, 4, 5]]).all())  # infinite gradients of dropped elements do not reach z
 
 
 def test_norms_repeat_bit_for_bit(cuda):
