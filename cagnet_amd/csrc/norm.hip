@@ -231,9 +231,9 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
   }
 }
 
-// dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added up.  One workgroup per 32
-// columns; 32 threads share a column, each adds every 32nd slice in order, then the 32 sums are added in order.
-constexpr int kFoldCols = 32, kFoldTeams = 32;
+// dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added up.  One workgroup per 16
+// columns; 64 threads share a column, each adds every 64th slice in order, then the 64 sums are added in order.
+constexpr int kFoldCols = 16, kFoldTeams = 64;
 
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kernel(NormArgs a, int32_t slices, void *dw_post,
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kerne
   const int64_t step = (int64_t)(RESIDUAL ? 2 : 1) * a.d;
   float q = 0.f, p = 0.f;
   if (j < a.d) {
-#pragma unroll 4
+#pragma unroll 8
     for (int32_t k = team; k < slices; k += kFoldTeams) {
       const float *at = a.partial + k * step + j;
       q += at[0];
