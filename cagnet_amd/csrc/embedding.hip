@@ -284,6 +284,8 @@ __global__ __launch_bounds__(kSortThreads) void emb_scatter_kernel(KeySource src
 // the table they belong to.  A row with more ("hot": with popular indices one can hold a tenth of all positions) covers
 // the end of at least one chunk, so a chunk holds a part of at most two hot rows, the one it begins in and the one it
 // ends in.  The team adds up each part into a partial row, and a second kernel adds a hot row's partial rows in order.
+// Where all chunks of a workgroup lie inside one hot row (padding can make one row hold half of all positions) their
+// sums are added in LDS first, and only the workgroup's first chunk has a partial row.
 // ---------------------------------------------------------------------------------------------
 struct Segment {
   int32_t from, to;  // sorted positions of one table row
@@ -302,6 +304,7 @@ struct SumArgs {
   int64_t ldo;
   float *partial;               // [2 * chunks][d], float32
   int32_t *hot_count, *hot;     // parts (2 * chunk + which) that hot rows begin with, in any order
+  int32_t teams;                // chunks of a workgroup
   unsigned chunk_groups;        // workgroups that stream; those behind them write the rows that no index names
 };
 
@@ -375,6 +378,7 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
   typedef typename Elem<DT>::type T;
   typedef typename Elem<OUT_F32 ? CG_F32 : DT>::type O;
   constexpr int V = Chunk<T, true>::V;
+  __shared__ float sums[kEmbThreads][V];
   const int lane = threadIdx.x & ((1 << lanes_log) - 1), teams = kEmbThreads >> lanes_log, team = threadIdx.x >> lanes_log;
   const int32_t j = ((int32_t)blockIdx.y * (1 << lanes_log) + lane) * V;
   if (blockIdx.x >= a.chunk_groups) {  // rows without positions
@@ -406,6 +410,24 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
   c.place(j, a.d);
   float *partial = a.partial + (int64_t)chunk * 2 * a.d + j;
   auto keep = [&](int32_t, float (&sum)[V]) { store_some<float, V>(partial, c.live, sum); };
+  const int32_t group = (int32_t)blockIdx.x * teams * a.span;
+  if (teams > 1 && first.from <= group && first.to - group >= teams * a.span) {  // of every thread alike; hot with two teams
+    stream_rows<T>(a, c, begin, end, [&](int32_t, float (&sum)[V]) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[threadIdx.x][i] = sum[i];
+    });
+    __syncthreads();
+    if (team != 0) return;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    for (int t = 0; t < teams; ++t)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += sums[(t << lanes_log) + lane][i];
+    keep(0, sum);
+    if (first.from == begin && lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
+    return;
+  }
   int32_t from = begin, to = last.to;  // of the light rows that begin here
   if (first.to - first.from > a.span) {
     from = first.to < end ? first.to : end;
@@ -441,12 +463,18 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
     const int32_t chunk = a.hot[h] >> 1, which = a.hot[h] & 1, begin = chunk * a.span;
     const int32_t end = all - begin < a.span ? all : begin + a.span;
     const int32_t v = a.key[which ? end - 1 : begin];
-    const int32_t stop = a.rowptr ? a.rowptr[v + 1] : a.ends[2 * chunk + which].to, parts = (stop - 1) / a.span - chunk + 1;
+    const Segment seg = a.rowptr ? Segment{a.rowptr[v], a.rowptr[v + 1]} : a.ends[2 * chunk + which];
+    // chunks with partial rows: those before the first whole workgroup of chunks, one of every whole workgroup, those behind
+    const int32_t wide = a.span * a.teams, tail = (seg.to - 1) / a.span;
+    int32_t lo = (seg.from + wide - 1) / wide, hi = seg.to / wide;
+    if (hi < lo) lo = hi = (chunk + a.teams - 1) / a.teams;
+    const int32_t head = lo * a.teams - chunk, whole = hi - lo, parts = head + whole + tail - hi * a.teams + 1;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     if (live > 0) {
 #pragma unroll 8
       for (int32_t k = wave; k < parts; k += kFoldWaves) {
-        const int64_t slot = (int64_t)(chunk + k) * 2 + (k == 0 ? which : 0);
+        const int32_t at = k < head ? chunk + k : k < head + whole ? (lo + k - head) * a.teams : hi * a.teams + k - head - whole;
+        const int64_t slot = (int64_t)at * 2 + (at == chunk ? which : 0);
         float f[4];
         load_some<float, 4>(a.partial + slot * a.d + j, live, f);
 #pragma unroll
@@ -593,7 +621,7 @@ static int check_lookup(const char *who, int64_t n, int64_t rows, int32_t d) {
   if (n < 0 || rows <= 0 || d <= 0)
     CG_FAIL(CG_ERR_SIZE, "%s: n=%lld indices into rows=%lld of d=%d elements", who, (long long)n, (long long)rows, d);
   if (d > (1 << 23)) CG_FAIL(CG_ERR_OVERFLOW, "%s: rows of d=%d elements (at most 2^23)", who, d);
-  if (n > 0x7fff0000LL || rows > 0x7ffffffdLL)
+  if (n > 0x7ff00000LL || rows > 0x7ffffffdLL)
     CG_FAIL(CG_ERR_OVERFLOW, "%s: n=%lld, rows=%lld overflow int32 positions", who, (long long)n, (long long)rows);
   return CG_OK;
 }
@@ -700,7 +728,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
     a.key = key[last], a.pos = pos[last], a.rowptr = rowptr, a.count = rowptr + rows;
   }
   const int per_chunk = dtype == CG_F32 ? 4 : 8, lanes_log = lanes_log2(d, per_chunk), teams = kEmbThreads >> lanes_log;
-  a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
+  a.teams = teams, a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
   int64_t groups = small || beta == 1.f ? 0 : ceil_div64(rows, teams);
   if (groups > 256 * 16) groups = 256 * 16;
   groups += a.chunk_groups;
