@@ -94,11 +94,22 @@ __device__ __forceinline__ int32_t key_at(const KeySource &s, int64_t i) {
   return (int32_t)(v >= 0 && v < s.rows ? v : s.rows);
 }
 
-// Counts of a tile's digits, at hist[digit * digit_step + tile * tile_step].
+struct Segment {
+  int32_t from, to;  // sorted positions of one table row; to == 0: none
+};
+
+// Counts of a tile's digits, at hist[digit * digit_step + tile * tile_step].  Workgroups behind the tiles clear the table
+// rows' segments meanwhile.
 __global__ __launch_bounds__(kSortThreads) void emb_hist_kernel(KeySource src, int64_t n, int shift, int dbits,
                                                                 uint32_t *__restrict__ hist, int64_t digit_step,
-                                                                int64_t tile_step) {
+                                                                int64_t tile_step, int64_t tiles,
+                                                                Segment *__restrict__ segments) {
   __shared__ uint32_t count[kMaxRadix];
+  if ((int64_t)blockIdx.x >= tiles) {
+    const int64_t step = (int64_t)(gridDim.x - tiles) * kSortThreads;
+    for (int64_t v = ((int64_t)blockIdx.x - tiles) * kSortThreads + threadIdx.x; v < src.rows; v += step) segments[v] = Segment{0, 0};
+    return;
+  }
   const int radix = 1 << dbits;
   if ((int)threadIdx.x < radix) count[threadIdx.x] = 0;
   const int64_t base = (int64_t)blockIdx.x * kSortTile;
@@ -277,6 +288,20 @@ __global__ __launch_bounds__(kSortThreads) void emb_scatter_kernel(KeySource src
   }
 }
 
+// The segments of the table rows that have positions, and how many positions are inside the table: one thread per place
+// between two sorted keys.  Rows without positions cost nothing here, however many of them lie between two keys.
+__global__ __launch_bounds__(kEmbThreads) void emb_segment_kernel(const int32_t *__restrict__ key, int32_t n, int32_t rows,
+                                                                  Segment *__restrict__ segments, int32_t *__restrict__ count) {
+  const int32_t i = (int32_t)((int64_t)blockIdx.x * kEmbThreads + threadIdx.x);
+  if (i > n) return;
+  const int32_t before = i > 0 ? key[i - 1] : -1, here = i < n ? key[i] : rows;
+  if (before != here) {
+    if (before >= 0) segments[before].to = i;
+    if (here < rows) segments[here].from = i;
+  }
+  if (before < rows && here == rows) *count = i;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Sums.  The sorted array is cut into chunks of `span` positions, one team of lanes each.  A table row with up to
 // `span` positions ("light") is added up and written by the team whose chunk it begins in, also where it ends behind
@@ -287,13 +312,10 @@ __global__ __launch_bounds__(kSortThreads) void emb_scatter_kernel(KeySource src
 // Where all chunks of a workgroup lie inside one hot row (padding can make one row hold half of all positions) their
 // sums are added in LDS first, and only the workgroup's first chunk has a partial row.
 // ---------------------------------------------------------------------------------------------
-struct Segment {
-  int32_t from, to;  // sorted positions of one table row
-};
 struct SumArgs {
   const void *g;
   int64_t ldg;
-  const int32_t *rowptr;  // first sorted position of every table row; nullptr after the one-launch sort, then `ends`
+  const Segment *segments;  // of every table row; nullptr after the one-launch sort, then `ends`
   const Segment *ends;    // of every chunk: the segments of its first and of its last position
   const int32_t *count;   // positions whose index is inside the table
   const int32_t *key, *pos;
@@ -387,7 +409,7 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
     if (left <= 0 || a.beta == 1.f) return;
     const int64_t step = (int64_t)(gridDim.x - a.chunk_groups) * teams;
     for (int64_t v = (int64_t)(blockIdx.x - a.chunk_groups) * teams + team; v < a.rows; v += step)
-      if (a.rowptr[v] == a.rowptr[v + 1]) {
+      if (a.segments[v].to == 0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) zero[i] = 0.f;
         put_row<O, V>(a, v, j, left < V ? left : V, zero);
@@ -398,10 +420,9 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
   if (chunk >= a.chunks || chunk * a.span >= all) return;
   const int32_t begin = chunk * a.span, end = all - begin < a.span ? all : begin + a.span;
   Segment first, last;
-  if (a.rowptr) {
-    const int32_t k0 = a.key[begin], k1 = a.key[end - 1];
-    first = Segment{a.rowptr[k0], a.rowptr[k0 + 1]};
-    last = Segment{a.rowptr[k1], a.rowptr[k1 + 1]};
+  if (a.segments) {
+    first = a.segments[a.key[begin]];
+    last = a.segments[a.key[end - 1]];
   } else {
     first = a.ends[2 * chunk];
     last = a.ends[2 * chunk + 1];
@@ -463,7 +484,7 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
     const int32_t chunk = a.hot[h] >> 1, which = a.hot[h] & 1, begin = chunk * a.span;
     const int32_t end = all - begin < a.span ? all : begin + a.span;
     const int32_t v = a.key[which ? end - 1 : begin];
-    const Segment seg = a.rowptr ? Segment{a.rowptr[v], a.rowptr[v + 1]} : a.ends[2 * chunk + which];
+    const Segment seg = a.segments ? a.segments[v] : a.ends[2 * chunk + which];
     // chunks with partial rows: those before the first whole workgroup of chunks, one of every whole workgroup, those behind
     const int32_t wide = a.span * a.teams, tail = (seg.to - 1) / a.span;
     int32_t lo = (seg.from + wide - 1) / wide, hi = seg.to / wide;
@@ -585,7 +606,7 @@ struct EmbPlan {
   int passes, dbits;
   int64_t tiles, chunks;
   int32_t span;
-  size_t key[2], pos[2], hist, totals, rowptr, ends, counters, hot, partial, bytes;  // offsets into the workspace
+  size_t key[2], pos[2], hist, totals, segments, ends, counters, hot, partial, bytes;  // offsets into the workspace
 };
 static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   EmbPlan p = {};
@@ -608,7 +629,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   for (int k = 0; k < 2; ++k) p.key[k] = take((size_t)n * 4), p.pos[k] = take((size_t)n * 4);
   p.hist = take((size_t)p.tiles * ((size_t)1 << p.dbits) * 4);
   p.totals = take((size_t)kMaxRadix * 4);
-  p.rowptr = take((size_t)(rows + 2) * 4);
+  p.segments = take((size_t)rows * sizeof(Segment));
   p.ends = take(p.tiles <= 1 ? (size_t)p.chunks * 2 * sizeof(Segment) : 0);
   p.counters = take(8);  // positions inside the table, hot rows
   p.hot = take((size_t)p.chunks * 4);
@@ -683,7 +704,8 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   int32_t *key[2] = {(int32_t *)(w + p.key[0]), (int32_t *)(w + p.key[1])};
   int32_t *pos[2] = {(int32_t *)(w + p.pos[0]), (int32_t *)(w + p.pos[1])};
   uint32_t *hist = (uint32_t *)(w + p.hist), *totals = (uint32_t *)(w + p.totals);
-  int32_t *rowptr = (int32_t *)(w + p.rowptr), *counters = (int32_t *)(w + p.counters);
+  Segment *segments = (Segment *)(w + p.segments);
+  int32_t *counters = (int32_t *)(w + p.counters);
   SumArgs a = {};
   a.g = d_g, a.ldg = ldg, a.count = counters, a.rows = rows, a.d = d, a.span = p.span, a.chunks = (int32_t)p.chunks;
   a.scale = scale, a.beta = beta, a.out = d_out, a.ldo = ldo, a.partial = (float *)(w + p.partial);
@@ -706,10 +728,17 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
     int last = 0;
     const bool direct = p.tiles <= kDirectTiles;
     const int radix = 1 << p.dbits;
+    int64_t clearing = ceil_div64(rows, kSortThreads * 4);
+    if (clearing > 1024) clearing = 1024;
+    if (n == 0) {
+      emb_hist_kernel<<<(unsigned)clearing, kSortThreads, 0, s>>>(src, 0, 0, p.dbits, hist, 0, 0, 0, segments);
+      CG_LAUNCH_CHECK();
+    }
     for (int pass = 0; n > 0 && pass < p.passes; ++pass) {
       const int to = pass & 1, shift = pass * p.dbits;
-      emb_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, direct ? 1 : p.tiles,
-                                                                 direct ? radix : 1);
+      const int64_t groups = p.tiles + (pass == 0 ? clearing : 0);
+      emb_hist_kernel<<<(unsigned)groups, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, direct ? 1 : p.tiles,
+                                                                direct ? radix : 1, p.tiles, segments);
       CG_LAUNCH_CHECK();
       if (direct) {
         emb_scatter_kernel<true><<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals,
@@ -724,8 +753,12 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
       src.key = key[to], src.pos = pos[to];
       last = to;
     }
-    CG_TRY(launch_rowptr(key[last], n, (int32_t)(rows + 1), rowptr, s));
-    a.key = key[last], a.pos = pos[last], a.rowptr = rowptr, a.count = rowptr + rows;
+    if (n > 0) {
+      emb_segment_kernel<<<(unsigned)ceil_div64(n + 1, kEmbThreads), kEmbThreads, 0, s>>>(key[last], (int32_t)n, (int32_t)rows,
+                                                                                          segments, counters);
+      CG_LAUNCH_CHECK();
+    }
+    a.key = key[last], a.pos = pos[last], a.segments = segments;
   }
   const int per_chunk = dtype == CG_F32 ? 4 : 8, lanes_log = lanes_log2(d, per_chunk), teams = kEmbThreads >> lanes_log;
   a.teams = teams, a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
