@@ -4,7 +4,8 @@ ReLU / log_softmax+NLL, forward and backward) on one AMD Instinct MI355X (gfx950
 Submodules
     ops                    tensor-level wrappers over the C ABI of lib/libcagnet_amd.so
     sparse_coo_tensor_cpp  the reference's native module, name for name (spmm_gpu, ...)
-    gcn                    broad_func / GCNFunc / train of the reference, restated for one GPU
+    gcn                    broad_func / GCNFunc / train of the reference, restated for one GPU; dropout, embedding,
+                           rms_norm and norm_residual with autograd
     synth                  seeded synthetic graphs and the reference's input preparation (pure torch)
     build                  hipcc recipe of the library
 

@@ -317,7 +317,8 @@ int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void 
 /* Its gradient, out_v = scale * sum_{i: idx_i = v} g_i + beta * out_v for every table row v (rows no index
  * names get beta * out_v, and are neither read nor written when beta == 1; beta == 0 never reads out).
  * out has the type of g or is float32 (`out_dtype`).  Indices outside the table add to nothing.  The
- * additions of a row run in a fixed order that depends on the indices alone. */
+ * additions of a row run in a fixed order that depends on the indices alone.  CG_ERR_OVERFLOW from
+ * 2^31 - 2^20 indices, 2^31 - 2 table rows or 2^23 + 1 columns on. */
 int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *bytes);
 int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64, int64_t n, int64_t rows, int32_t d,
                      int dtype, int out_dtype, float scale, float beta, void *d_out, int64_t ldo, void *d_work,
