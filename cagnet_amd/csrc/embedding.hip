@@ -203,6 +203,8 @@ __device__ __forceinline__ uint32_t sort_tile(SortLds &s, const int32_t (&key)[k
     if (valid) had = s.count[wave][digit];
     // the lowest lane of the set writes the new count; it depends on `had`, so the read above comes first
     if (valid && lower == 0) s.count[wave][digit] = had + (uint32_t)__popcll(peers);
+    // LDS serves a wavefront in order; the fence holds the compiler to it (it emits nothing)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     rank[r] = had + lower;
   }
   __syncthreads();
@@ -697,7 +699,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   if (ldo < d || (n > 0 && ldg < d)) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
   if (d_out == d_g) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the input", who);
   const EmbPlan p = emb_plan(n, rows, d);
-  if (work_bytes < (int64_t)p.bytes) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)p.bytes);
+  CG_TRY(check_work(who, d_work, work_bytes, (int64_t)p.bytes));
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof("embedding_bwd", d, s);
   char *w = static_cast<char *>(d_work);

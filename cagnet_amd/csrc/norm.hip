@@ -288,6 +288,13 @@ static size_t norm_workspace(int64_t n, int32_t d) {
   return (size_t)slices * (size_t)d * sizeof(float);
 }
 
+// columns are stepped through in int32, a workgroup's width at a time
+static int check_norm_shape(const char *who, int64_t n, int32_t d) {
+  CG_TRY(check_row_shape(who, n, d));
+  if (d > (1 << 30)) CG_FAIL(CG_ERR_OVERFLOW, "%s: rows of d=%d elements (at most 2^30)", who, d);
+  return CG_OK;
+}
+
 static int check_weights(const char *who, int dtype, int wdtype) {
   if (wdtype != CG_F32 && wdtype != dtype)
     CG_FAIL(CG_ERR_UNSUPPORTED, "%s: weights of dtype %d beside activations of dtype %d (CG_F32 or the same)", who, wdtype, dtype);
@@ -340,7 +347,7 @@ extern "C" {
 int cg_norm_bwd_workspace(int64_t n, int32_t d, int64_t *bytes) {
   using namespace cg;
   if (!bytes) CG_FAIL(CG_ERR_NULL, "cg_norm_bwd_workspace: null pointer");
-  CG_TRY(check_row_shape("cg_norm_bwd_workspace", n, d));
+  CG_TRY(check_norm_shape("cg_norm_bwd_workspace", n, d));
   *bytes = (int64_t)norm_workspace(n, d);
   return CG_OK;
 }
@@ -351,7 +358,7 @@ int cg_rms_norm_fwd(const void *d_x, int64_t ldx, const void *d_w, int wdtype, v
   const char *who = "cg_rms_norm_fwd";
   CG_TRY(check_dtype(who, dtype));
   CG_TRY(check_weights(who, dtype, wdtype));
-  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_norm_shape(who, n, d));
   CG_TRY(check_float(who, "eps", eps, true));
   if (n == 0) return CG_OK;
   if (!d_x || !d_y || !d_rstd) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
@@ -371,12 +378,12 @@ int cg_rms_norm_bwd(const void *d_g, int64_t ldg, const void *d_x, int64_t ldx, 
   const char *who = "cg_rms_norm_bwd";
   CG_TRY(check_dtype(who, dtype));
   CG_TRY(check_weights(who, dtype, wdtype));
-  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_norm_shape(who, n, d));
   if (n > 0) {
     if (!d_g || !d_x || !d_rstd || !d_dx || !d_work) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
     if (ldg < d || ldx < d || lddx < d) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
     if (d_dx == d_g || d_dx == d_x) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be an input", who);
-    if (work_bytes < (int64_t)norm_workspace(n, d)) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)norm_workspace(n, d));
+    CG_TRY(check_work(who, d_work, work_bytes, (int64_t)norm_workspace(n, d)));
   }
   NormArgs a = {};
   a.dh = d_g, a.lddh = ldg, a.z = d_x, a.ldz = ldx, a.w_post = d_w, a.w_f32 = wdtype == CG_F32;
@@ -395,7 +402,7 @@ int cg_norm_residual_fwd(const void *d_z, int64_t ldz, const void *d_x, int64_t 
   const char *who = "cg_norm_residual_fwd";
   CG_TRY(check_dtype(who, dtype));
   CG_TRY(check_weights(who, dtype, wdtype));
-  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_norm_shape(who, n, d));
   CG_TRY(check_float(who, "eps", eps, true));
   CG_TRY(check_float(who, "alpha", alpha, false));
   CG_TRY(check_p(who, p, d_rng));
@@ -427,7 +434,7 @@ int cg_norm_residual_bwd(const void *d_dr, int64_t lddr, const void *d_dh, int64
   const char *who = "cg_norm_residual_bwd";
   CG_TRY(check_dtype(who, dtype));
   CG_TRY(check_weights(who, dtype, wdtype));
-  CG_TRY(check_row_shape(who, n, d));
+  CG_TRY(check_norm_shape(who, n, d));
   CG_TRY(check_float(who, "alpha", alpha, false));
   CG_TRY(check_p(who, p, d_rng));
   if (gate_kind < CG_GATE_NONE || gate_kind > CG_GATE_FULL) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: gate kind %d", who, gate_kind);
@@ -445,7 +452,7 @@ int cg_norm_residual_bwd(const void *d_dr, int64_t lddr, const void *d_dh, int64
         if (outs[o] && outs[o] == i) CG_FAIL(CG_ERR_ALIAS, "%s: an output may not be an input", who);
       if (outs[o] && outs[o] == outs[(o + 1) % 3]) CG_FAIL(CG_ERR_ALIAS, "%s: two outputs are the same", who);
     }
-    if (work_bytes < (int64_t)norm_workspace(n, d)) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)work_bytes, (long long)norm_workspace(n, d));
+    CG_TRY(check_work(who, d_work, work_bytes, (int64_t)norm_workspace(n, d)));
   }
   NormArgs a = {};
   a.dr = d_dr, a.lddr = lddr, a.dh = d_dh, a.lddh = lddh, a.z = d_z, a.ldz = ldz, a.r_in = d_r, a.ldr_in = ldr;

@@ -174,7 +174,7 @@ __device__ __forceinline__ void weight_put(void *w, int w_f32, int32_t j, float 
   if (w_f32)
     static_cast<float *>(w)[j] = v;
   else
-    static_cast<T *>(w)[j] = (T)v;
+    static_cast<T *>(w)[j] = rounded<T>(v);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -271,6 +271,11 @@ static inline int check_dtype(const char *who, int dtype) {
 static inline int check_row_shape(const char *who, int64_t n, int32_t d) {
   if (n < 0 || d <= 0) CG_FAIL(CG_ERR_SIZE, "%s: n=%lld rows of d=%d elements", who, (long long)n, d);
   if (n > 0xffffffffLL) CG_FAIL(CG_ERR_OVERFLOW, "%s: n=%lld rows (at most 2^32 - 1)", who, (long long)n);
+  return CG_OK;
+}
+static inline int check_work(const char *who, const void *d_work, int64_t have, int64_t need) {
+  if (have < need) CG_FAIL(CG_ERR_SIZE, "%s: workspace of %lld bytes, %lld needed", who, (long long)have, (long long)need);
+  if ((uintptr_t)d_work % 16 != 0) CG_FAIL(CG_ERR_UNSUPPORTED, "%s: the workspace is not 16-byte aligned", who);
   return CG_OK;
 }
 static inline int check_p(const char *who, double p, const int64_t *d_rng) {

@@ -502,6 +502,8 @@ def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, 
     hidden activations between the two layers (the reference has none); `rng` is then the generator state
     (`rng_state`), which every epoch steps once."""
     g1, g2 = group if isinstance(group, (tuple, list)) else (group, group)
+    if not 0.0 <= dropout_p <= 1.0:
+        raise ValueError(f"train: dropout probability {dropout_p} outside [0, 1]")
     if dropout_p > 0.0 and rng is None:
         raise ValueError("train: dropout_p > 0 needs a generator state (rng)")
     outputs = GCNFunc.apply(inputs, weight1, adj_matrix, am_partitions, rank, size, g1, F.relu)

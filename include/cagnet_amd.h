@@ -286,7 +286,7 @@ int cg_log_softmax_nll_fwd(const float *d_z, int64_t ldz, const int64_t *d_y, co
  * them (no counterpart; its layers end in F.relu / F.log_softmax, gcn_distr.py:284-294).
  * Arithmetic is float32 whatever the type, rounded once at each store.  Weight vectors ([d], NULL =
  * ones) and their gradients are float32 or have the activations' type (`wdtype`, one for all).
- * n rows (at most 2^32 - 1) of d columns; n == 0 is legal (weight gradients are then zero).
+ * n rows (at most 2^32 - 1) of d columns (norms: at most 2^30); n == 0 is legal (weight gradients are then zero).
  * Outputs may not overlap inputs (cg_dropout may run in place).  Nothing is allocated and nothing is
  * read back: the gradients that need temporary memory take it from the caller (`d_work`, at least the
  * size the matching *_workspace function names, 16-byte aligned), so that every call can be captured

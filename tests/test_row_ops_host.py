@@ -169,3 +169,24 @@ def test_python_surface_refuses_cpu_tensors_and_wrong_types():
     state = ops.rng_state(-5, "cpu", offset=(1 << 64) - 1)
     assert state.tolist() == [-5, -1]
     assert ops.rng_state((1 << 63) + 9, "cpu").tolist() == [-(1 << 63) + 9, 0]
+
+
+def test_refusals_of_workspaces_widths_and_probabilities():
+    from cagnet_amd import gcn
+
+    lib, a, b, c, e = _lib(), 16, 4096, 8192, 16384
+    size, wide = ctypes.c_int64(-1), (1 << 30) + 1
+    for off in (1, 4, 8):  # a workspace that is not 16-byte aligned
+        assert lib.cg_embedding_bwd(a, 8, b, 1, 5, 4, 8, F32, F32, 1.0, 0.0, c, 8, e + off, 1 << 20, None) == UNSUPPORTED
+        assert lib.cg_rms_norm_bwd(a, 8, b, 8, None, F32, c, e, 8, None, 5, 8, F32, c + off, 1 << 20, None) == UNSUPPORTED
+        assert lib.cg_norm_residual_bwd(a, 8, b, 8, c, 8, e, 8, None, 8, 0, None, None, None, F32, 1.0, 0.0, None, a, a, 32768, 8,
+                                        65536, 8, None, 8, None, None, None, 5, 8, F32, a + off, 1 << 20, None) == UNSUPPORTED
+    # rows of more elements than the norms count
+    assert lib.cg_norm_bwd_workspace(1, wide, ctypes.byref(size)) == OVERFLOW
+    assert lib.cg_norm_bwd_workspace(1, wide - 1, ctypes.byref(size)) == 0
+    assert lib.cg_rms_norm_fwd(a, wide, None, F32, b, wide, c, 1, wide, F32, 1e-6, None) == OVERFLOW
+    assert lib.cg_embedding_fwd(a, wide, 1, b, 1, 1, wide, F32, 1.0, c, wide, None) == OVERFLOW
+    x = torch.zeros(4, 8)
+    for p in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError, match="outside"):
+            gcn.train(x, x, x, 4, [], None, None, dropout_p=p, rng=torch.zeros(2, dtype=torch.int64))
