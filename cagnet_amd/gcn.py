@@ -14,6 +14,7 @@ Names and argument order follow the reference so that its drivers read the same.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import List, Optional, Sequence, Union
 
@@ -395,6 +396,18 @@ class LogSoftmaxNLLLoss(torch.autograd.Function):
 rng_state, rng_next = ops.rng_state, ops.rng_next
 
 
+def _first_order(backward):
+    """A backward pass without a gradient of its own.  The engine turns recording off unless create_graph asks for it;
+    only then the wrapper that refuses second derivatives is needed (a step of a few rows is bound by the host)."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 class Dropout(torch.autograd.Function):
     """ops.dropout_fwd / dropout_bwd; only the generator's snapshot is kept between them."""
 
@@ -405,7 +418,7 @@ class Dropout(torch.autograd.Function):
         return ops.dropout_fwd(x, p, rng)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         return ops.dropout_bwd(g, ctx.p, ctx.saved_tensors[0] if ctx.has_rng else None), None, None
 
@@ -428,7 +441,7 @@ class Embedding(torch.autograd.Function):
         return out if idx.dim() == 1 else out.view(*idx.shape, table.shape[1])
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         (flat,) = ctx.saved_tensors
         g = g if g.dim() == 2 else g.reshape(-1, ctx.width)
@@ -450,7 +463,7 @@ class RmsNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         x, rstd, *weight = ctx.saved_tensors
         dx, dw = ops.rms_norm_bwd(g, x, weight[0] if weight else None, rstd)
@@ -476,7 +489,7 @@ class NormResidual(torch.autograd.Function):
         return r, h
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dr, dh):
         if dr is None and dh is None:
             return (None,) * 10

@@ -713,6 +713,11 @@ def _row_stats(t: torch.Tensor, name: str, x: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A result shaped as the activation t, rows side by side (empty_like is cheaper than empty on the host)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _at(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -768,7 +773,7 @@ def _dropout(x: torch.Tensor, p: float, rng: Optional[torch.Tensor], name: str) 
     x, ldx = _rows(x, name)
     p = _probability(p, rng, x)
     n, d = x.shape
-    out = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    out = _like(x)
     _run(x.device, "cg_dropout", lib.cg_dropout, x.data_ptr(), ldx, out.data_ptr(), d, n, d, _ROW_DTYPES[x.dtype], p, _at(rng))
     return out
 
@@ -802,7 +807,7 @@ def embedding_fwd(table: torch.Tensor, idx: torch.Tensor, scale: float = 1.0) ->
     idx = _lookup_indices(idx, table.device)
     rows, d = table.shape
     n = idx.shape[0]
-    out = torch.empty((n, d), dtype=table.dtype, device=table.device)
+    out = table.new_empty((n, d))
     _run(table.device, "cg_embedding_fwd", lib.cg_embedding_fwd, table.data_ptr(), ldt, rows, idx.data_ptr(),
          idx.dtype == torch.int64, n, d, _ROW_DTYPES[table.dtype], scale, out.data_ptr(), d)
     return out
@@ -845,7 +850,7 @@ def rms_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1
     x, ldx = _rows(x, "x")
     w, wdtype = _weights(x, weight=weight)
     n, d = x.shape
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    y = _like(x)
     rstd = torch.empty(n, dtype=torch.float32, device=x.device)
     _run(x.device, "cg_rms_norm_fwd", lib.cg_rms_norm_fwd, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype], y.data_ptr(), d,
          rstd.data_ptr(), n, d, _ROW_DTYPES[x.dtype], eps)
@@ -859,7 +864,7 @@ def rms_norm_bwd(g: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor
     w, wdtype = _weights(x, weight=weight)
     rstd = _row_stats(rstd, "rstd", x)
     n, d = x.shape
-    dx = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    dx = _like(x)
     dw = torch.empty_like(w) if w is not None else None
     work = _workspace("cg_norm_bwd_workspace", x.device, n, d)
     _run(x.device, "cg_rms_norm_bwd", lib.cg_rms_norm_bwd, g.data_ptr(), ldg, x.data_ptr(), ldx, _at(w), _ROW_DTYPES[wdtype],
@@ -892,8 +897,7 @@ def norm_residual_fwd(z: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.T
     w_post, w_pre, scale, wdtype = _weights(z, w_post=w_post, w_pre=w_pre, scale=scale)
     p = _probability(p, rng, z)
     n, d = z.shape
-    r = torch.empty((n, d), dtype=z.dtype, device=z.device)
-    h = torch.empty_like(r)
+    r, h = _like(z), _like(z)
     rstd_z = torch.empty(n, dtype=torch.float32, device=z.device)
     rstd_r = torch.empty_like(rstd_z)
     _run(z.device, "cg_norm_residual_fwd", lib.cg_norm_residual_fwd, z.data_ptr(), ldz, x.data_ptr(), ldx, _at(gate), ldg,
@@ -922,9 +926,8 @@ def norm_residual_bwd(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], z:
     rstd_z, rstd_r = _row_stats(rstd_z, "rstd_z", z), _row_stats(rstd_r, "rstd_r", z)
     p = _probability(p, rng, z)
     n, d = z.shape
-    dz = torch.empty((n, d), dtype=z.dtype, device=z.device)
-    dx = torch.empty_like(dz)
-    dgate = torch.empty(gate.shape, dtype=z.dtype, device=z.device) if gate is not None else None
+    dz, dx = _like(z), _like(z)
+    dgate = _like(gate) if gate is not None else None
     dw_post, dw_pre, dscale = (torch.empty_like(w) if w is not None else None for w in (w_post, w_pre, scale))
     work = _workspace("cg_norm_bwd_workspace", z.device, n, d)
     _run(z.device, "cg_norm_residual_bwd", lib.cg_norm_residual_bwd, _at(dr), lddr, _at(dh), lddh, z.data_ptr(), ldz,

@@ -726,3 +726,44 @@ def test_graphed_train_with_dropout_equals_eager(cuda):
     assert torch.allclose(g1, w1, atol=1e-5) and torch.allclose(g2, w2, atol=1e-5)
     assert state.tolist() == [4, 8]
     graphed.close()
+
+
+@pytest.mark.parametrize("op", ["dropout", "embedding", "rms_norm", "norm_residual"])
+def test_second_derivatives_are_refused_first_ones_are_the_same(cuda, op):
+    from cagnet_amd import gcn, ops
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, z = (torch.randn(33, 20, device="cuda", generator=gen).requires_grad_() for _ in range(2))
+    w = torch.randn(20, device="cuda", generator=gen).requires_grad_()
+    g = torch.randn(33, 20, device="cuda", generator=gen).requires_grad_()
+    idx = torch.randint(0, 33, (33,), device="cuda", generator=gen)
+    rng = ops.rng_state(3)
+    call, leaf = {"dropout": (lambda: gcn.dropout(x, 0.3, rng), x), "embedding": (lambda: gcn.embedding(x, idx, 2.0), x),
+                  "rms_norm": (lambda: gcn.rms_norm(x, w), x),
+                  "norm_residual": (lambda: gcn.norm_residual(z, x, w, w, p=0.3, rng=rng)[1], z)}[op]
+    (want,) = torch.autograd.grad(call(), leaf, g)
+    (got,) = torch.autograd.grad(call(), leaf, g, create_graph=True)
+    assert not want.requires_grad and torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got.sum().backward()
+
+
+@pytest.mark.parametrize("n, d", [(1, 24), (7, 1), (1, 1), (6, 24)])
+def test_results_are_contiguous_whatever_the_strides(cuda, n, d):
+    from cagnet_amd import ops
+
+    wide = torch.randn(d, 3 * n, device="cuda").t()[::3]      # columns apart, rows apart
+    apart = torch.randn(n, 40, device="cuda")[:, :d]          # rows apart
+    w = torch.randn(d, device="cuda")
+    for x in (wide, apart):
+        y, rstd = ops.rms_norm_fwd(x, w)
+        dx, _ = ops.rms_norm_bwd(x, x, w, rstd)
+        r, h, rz, rr = ops.norm_residual_fwd(x, x, w, w, gate=x)
+        outs = [ops.dropout_fwd(x, 0.0, None), y, dx, r, h, *ops.norm_residual_bwd(x, x, x, r, w, w, rz, rr, gate=x)[:3]]
+        assert all(o.is_contiguous() and o.shape == x.shape for o in outs)
+        x = x.contiguous()
+        y2, rstd = ops.rms_norm_fwd(x, w)
+        r2, h2, rz, rr = ops.norm_residual_fwd(x, x, w, w, gate=x)
+        same = [x, y2, ops.rms_norm_bwd(x, x, w, rstd)[0], r2, h2,
+                *ops.norm_residual_bwd(x, x, x, r2, w, w, rz, rr, gate=x)[:3]]
+        assert all(torch.equal(a, b) for a, b in zip(outs, same))
