@@ -35,14 +35,14 @@ static inline int lanes_log2(int32_t d, int per_chunk) {
 // ---------------------------------------------------------------------------------------------
 constexpr int kLookups = 4;
 
-template <int DT>
+template <int DT, int FIT>
 __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typename Elem<DT>::type *__restrict__ table,
                                                                     int64_t ldt, int64_t rows, IndexView idx, int64_t n,
                                                                     int32_t d, float scale, int lanes_log,
                                                                     typename Elem<DT>::type *__restrict__ out,
                                                                     int64_t ldo) {
   typedef typename Elem<DT>::type T;
-  typedef Chunk<T, true> C;
+  typedef Span<T, FIT> C;
   const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1), teams = kEmbThreads >> lanes_log;
   const int64_t step = (int64_t)gridDim.x * teams * kLookups;
   for (int64_t i0 = ((int64_t)blockIdx.x * teams + (threadIdx.x >> lanes_log)) * kLookups; i0 < n; i0 += step) {
@@ -349,11 +349,33 @@ __device__ __forceinline__ void put_row(const SumArgs &a, int64_t v, int32_t j, 
   store_some<O, V>(out, live, sum);
 }
 
-// Adds up the chunk's columns of g's rows pos[from .. to) in order, one sum per stretch of equal keys, and hands each
+// The same for a lane's 16 bytes of g's type: stored whole where nothing is read back, the elements that count otherwise
+// (a repeated element would be read after the lane before has written it).
+template <typename O, typename C>
+__device__ __forceinline__ void put_span(const SumArgs &a, const C &c, int64_t v, float (&sum)[C::V]) {
+  O *out = (O *)a.out + v * a.ldo + c.at;
+#pragma unroll
+  for (int i = 0; i < C::V; ++i) sum[i] *= a.scale;
+  if (c.whole() && (a.beta == 0.f || c.dup == 0)) {
+    if (a.beta != 0.f) {
+      float old[C::V];
+      load_pack<O, C::V>(out, old);
+#pragma unroll
+      for (int i = 0; i < C::V; ++i) sum[i] += a.beta * old[i];
+    }
+    store_pack<O, C::V>(out, sum);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < C::V; ++i)
+    if (c.counts(i)) out[i] = rounded<O>(a.beta != 0.f ? sum[i] + a.beta * (float)out[i] : sum[i]);
+}
+
+// Adds up the lane's columns of g's rows pos[from .. to) in order, one sum per stretch of equal keys, and hands each
 // to done(key, sum).  The positions and keys of the next kAhead rows are loaded while those before are on their way.
-template <typename T, typename F>
-__device__ __forceinline__ void stream_rows(const SumArgs &a, const Chunk<T, true> &c, int32_t from, int32_t to, F done) {
-  constexpr int V = Chunk<T, true>::V;
+template <typename T, typename C, typename F>
+__device__ __forceinline__ void stream_rows(const SumArgs &a, const C &c, int32_t from, int32_t to, F done) {
+  constexpr int V = C::V;
   if (from >= to) return;
   int32_t p[kAhead], key[kAhead], next[kAhead];
 #pragma unroll
@@ -397,24 +419,26 @@ __device__ __forceinline__ void stream_rows(const SumArgs &a, const Chunk<T, tru
   done(now, sum);
 }
 
-template <int DT, bool OUT_F32>
+template <int DT, bool OUT_F32, int FIT>
 __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lanes_log) {
   typedef typename Elem<DT>::type T;
   typedef typename Elem<OUT_F32 ? CG_F32 : DT>::type O;
-  constexpr int V = Chunk<T, true>::V;
+  typedef Span<T, FIT> C;
+  constexpr int V = C::V;
   __shared__ float sums[kEmbThreads][V];
   const int lane = threadIdx.x & ((1 << lanes_log) - 1), teams = kEmbThreads >> lanes_log, team = threadIdx.x >> lanes_log;
   const int32_t j = ((int32_t)blockIdx.y * (1 << lanes_log) + lane) * V;
+  C c;
+  c.place(j, a.d);
   if (blockIdx.x >= a.chunk_groups) {  // rows without positions
     float zero[V];
-    const int32_t left = a.d - j;
-    if (left <= 0 || a.beta == 1.f) return;
+    if (!c.any() || a.beta == 1.f) return;
     const int64_t step = (int64_t)(gridDim.x - a.chunk_groups) * teams;
     for (int64_t v = (int64_t)(blockIdx.x - a.chunk_groups) * teams + team; v < a.rows; v += step)
       if (a.segments[v].to == 0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) zero[i] = 0.f;
-        put_row<O, V>(a, v, j, left < V ? left : V, zero);
+        put_span<O>(a, c, v, zero);
       }
     return;
   }
@@ -429,10 +453,18 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
     first = a.ends[2 * chunk];
     last = a.ends[2 * chunk + 1];
   }
-  Chunk<T, true> c;
-  c.place(j, a.d);
-  float *partial = a.partial + (int64_t)chunk * 2 * a.d + j;
-  auto keep = [&](int32_t, float (&sum)[V]) { store_some<float, V>(partial, c.live, sum); };
+  const bool hot_first = first.to - first.from > a.span, hot_last = last.to - last.from > a.span;
+  const int32_t first_key = a.key[begin], last_key = a.key[end - 1];
+  float *partial = a.partial + (int64_t)chunk * 2 * a.d + c.at;
+  auto keep = [&](float *to, const float (&sum)[V]) {
+    if (FIT != kShortRow) {
+      store_pack<float, V>(to, sum);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (c.counts(i)) to[i] = sum[i];
+    }
+  };
   const int32_t group = (int32_t)blockIdx.x * teams * a.span;
   if (teams > 1 && first.from <= group && first.to - group >= teams * a.span) {  // of every thread alike; hot with two teams
     stream_rows<T>(a, c, begin, end, [&](int32_t, float (&sum)[V]) {
@@ -447,43 +479,42 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
     for (int t = 0; t < teams; ++t)
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += sums[(t << lanes_log) + lane][i];
-    keep(0, sum);
+    if (c.any()) keep(partial, sum);
     if (first.from == begin && lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
     return;
   }
-  int32_t from = begin, to = last.to;  // of the light rows that begin here
-  if (first.to - first.from > a.span) {
-    from = first.to < end ? first.to : end;
-    stream_rows<T>(a, c, begin, from, keep);
-    if (first.from == begin && lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
-  } else if (first.from < begin) {
-    from = first.to;
+  if (lane == 0 && blockIdx.y == 0) {
+    if (hot_first && first.from == begin) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
+    if (hot_last && last.from > begin) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk + 1;
   }
-  if (last.to - last.from > a.span) {
-    to = last.from;  // at or before `from` where it is the first one too
-    if (last.from > begin) {
-      partial += a.d;
-      stream_rows<T>(a, c, last.from, end, keep);
-      if (lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk + 1;
-    }
-  }
-  if (from < end)
-    stream_rows<T>(a, c, from, to, [&](int32_t v, float (&sum)[V]) { put_row<O, V>(a, v, j, c.live, sum); });
+  // a light row that began in the chunk before is that chunk's, one that begins here is followed behind the end
+  const int32_t from = !hot_first && first.from < begin ? first.to : begin, to = hot_last ? end : last.to;
+  stream_rows<T>(a, c, from, to, [&](int32_t v, float (&sum)[V]) {
+    if (!c.any()) return;
+    if (hot_first && v == first_key)
+      keep(partial, sum);
+    else if (hot_last && v == last_key)
+      keep(partial + a.d, sum);
+    else
+      put_span<O>(a, c, v, sum);
+  });
 }
 
-// The partial rows of the hot rows, 256 columns a workgroup: its 16 wavefronts take every 16th partial row each, their
-// sums are added in order.
+// The partial rows of the hot rows, 256 columns a workgroup (of as many hot rows side by side as these hold): its 16
+// wavefronts take every 16th partial row each, their sums are added in order.
 constexpr int kFoldWaves = 16, kFoldColumns = kWave * 4;
 
 template <int OT>
-__global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) {
+__global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a, int lanes_log) {
   typedef typename Elem<OT>::type O;
   __shared__ float lds[kFoldWaves][kFoldColumns];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int32_t j = blockIdx.y * kFoldColumns + lane * 4, all = *a.count, hot = *a.hot_count;
+  const int team = lane >> lanes_log, teams = kWave >> lanes_log;
+  const int32_t j = blockIdx.y * kFoldColumns + (lane & ((1 << lanes_log) - 1)) * 4, all = *a.count, hot = *a.hot_count;
   const int live = a.d - j < 4 ? a.d - j : 4;
-  for (int32_t h = blockIdx.x; h < hot; h += gridDim.x) {  // uniform in the workgroup
-    const int32_t chunk = a.hot[h] >> 1, which = a.hot[h] & 1, begin = chunk * a.span;
+  for (int32_t h0 = blockIdx.x * teams; h0 < hot; h0 += gridDim.x * teams) {  // uniform in the workgroup
+    const int32_t part = a.hot[h0 + team < hot ? h0 + team : h0], chunk = part >> 1, which = part & 1, begin = chunk * a.span;
+    const bool mine = h0 + team < hot && live > 0;
     const int32_t end = all - begin < a.span ? all : begin + a.span;
     const int32_t v = a.key[which ? end - 1 : begin];
     const Segment seg = a.segments ? a.segments[v] : a.ends[2 * chunk + which];
@@ -493,7 +524,7 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
     if (hi < lo) lo = hi = (chunk + a.teams - 1) / a.teams;
     const int32_t head = lo * a.teams - chunk, whole = hi - lo, parts = head + whole + tail - hi * a.teams + 1;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live > 0) {
+    if (mine) {
 #pragma unroll 8
       for (int32_t k = wave; k < parts; k += kFoldWaves) {
         const int32_t at = k < head ? chunk + k : k < head + whole ? (lo + k - head) * a.teams : hi * a.teams + k - head - whole;
@@ -504,11 +535,11 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a) 
         for (int i = 0; i < 4; ++i) sum[i] += f[i];
       }
     }
-    __syncthreads();  // the sums of the row before have been read
+    __syncthreads();  // the sums of the rows before have been read
 #pragma unroll
     for (int i = 0; i < 4; ++i) lds[wave][lane * 4 + i] = sum[i];
     __syncthreads();
-    if (wave != 0 || live <= 0) continue;
+    if (wave != 0 || !mine) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum[i] = 0.f;
@@ -669,10 +700,19 @@ int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void 
   int64_t groups = ceil_div64(n, (int64_t)(kEmbThreads >> lanes_log) * kLookups);
   if (groups > 256 * 64) groups = 256 * 64;
   const IndexView view = {d_idx, idx64 != 0};
-#define CG_CALL(DT)                                                                                              \
-  embedding_fwd_kernel<DT><<<(unsigned)groups, kEmbThreads, 0, s>>>((const Elem<DT>::type *)d_table, ldt, rows, view, n, \
-                                                                     d, scale, lanes_log, (Elem<DT>::type *)d_out, ldo)
+  const int32_t v = dtype == CG_F32 ? 4 : 8;
+#define CG_FIT(DT, FIT)                                                                                                   \
+  embedding_fwd_kernel<DT, FIT><<<(unsigned)groups, kEmbThreads, 0, s>>>((const Elem<DT>::type *)d_table, ldt, rows, view, \
+                                                                          n, d, scale, lanes_log, (Elem<DT>::type *)d_out, ldo)
+#define CG_CALL(DT)              \
+  if (d % v == 0)                \
+    CG_FIT(DT, kWholeChunks);    \
+  else if (d < v)                \
+    CG_FIT(DT, kShortRow);       \
+  else                           \
+    CG_FIT(DT, kPartChunk)
   CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_FIT
 #undef CG_CALL
   CG_LAUNCH_CHECK();
   return CG_OK;
@@ -769,17 +809,28 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   groups += a.chunk_groups;
   if (groups == 0) return CG_OK;
   const dim3 grid((unsigned)groups, (unsigned)ceil_div64(d, (int64_t)per_chunk << lanes_log));
-#define CG_CALL(DT)                                                      \
-  if (out_dtype == CG_F32)                                               \
-    emb_sum_kernel<DT, true><<<grid, kEmbThreads, 0, s>>>(a, lanes_log); \
-  else                                                                   \
-    emb_sum_kernel<DT, false><<<grid, kEmbThreads, 0, s>>>(a, lanes_log)
+#define CG_FIT(DT, FIT)                                                       \
+  if (out_dtype == CG_F32)                                                    \
+    emb_sum_kernel<DT, true, FIT><<<grid, kEmbThreads, 0, s>>>(a, lanes_log); \
+  else                                                                        \
+    emb_sum_kernel<DT, false, FIT><<<grid, kEmbThreads, 0, s>>>(a, lanes_log)
+#define CG_CALL(DT)               \
+  if (d % per_chunk == 0) {       \
+    CG_FIT(DT, kWholeChunks);     \
+  } else if (d < per_chunk) {     \
+    CG_FIT(DT, kShortRow);        \
+  } else {                        \
+    CG_FIT(DT, kPartChunk);       \
+  }
   CG_BY_DTYPE(dtype, CG_CALL)
+#undef CG_FIT
 #undef CG_CALL
   CG_LAUNCH_CHECK();
   if (n <= p.span) return CG_OK;  // no row can be hot
   const dim3 fold((unsigned)(p.chunks < 512 ? p.chunks : 512), (unsigned)ceil_div64(d, kFoldColumns));
-#define CG_CALL(OT) emb_fold_kernel<OT><<<fold, kWave * kFoldWaves, 0, s>>>(a)
+  int fold_lanes_log = lanes_log2(d, 4);
+  if (fold_lanes_log > 6) fold_lanes_log = 6;
+#define CG_CALL(OT) emb_fold_kernel<OT><<<fold, kWave * kFoldWaves, 0, s>>>(a, fold_lanes_log)
   CG_BY_DTYPE(out_dtype, CG_CALL)
 #undef CG_CALL
   CG_LAUNCH_CHECK();
