@@ -31,7 +31,8 @@ static inline int lanes_log2(int32_t d, int per_chunk) {
 // ---------------------------------------------------------------------------------------------
 // lookup: kLookups rows a team at once, all indices loaded before the first row and all rows before the first store.
 // Bound by memory: 131,072 x 1024 float32 from 65,536 rows 173 us = 4.7 TB/s of rows read once and written (185 us with
-// two rows at once, 173 with eight); 232,965 x 128 from 50,021 rows 28 us (28 and 29 us).
+// two rows at once, 173 with eight); 232,965 x 128 from 50,021 rows 28 us (28 and 29 us).  Rows that end inside 16 bytes
+// take them whole too: 605,100 x 55 float16 22 us, 36 with the last ones shifted and stored one by one.
 // ---------------------------------------------------------------------------------------------
 constexpr int kLookups = 4;
 
@@ -97,6 +98,10 @@ __device__ __forceinline__ int32_t key_at(const KeySource &s, int64_t i) {
 struct Segment {
   int32_t from, to;  // sorted positions of one table row; to == 0: none
 };
+
+// Hot rows are listed by one atomic each; kHotLists counters in cache lines of their own share them, because atomics on one
+// address follow each other at 25 ns (1,000,000 x 60 float32 popular indices: 126 us with one counter, 116 with eight; in chunks of 8 434 and 139).
+constexpr int kHotLists = 8, kHotStride = 64;
 
 // Counts of a tile's digits, at hist[digit * digit_step + tile * tile_step].  Workgroups behind the tiles clear the table
 // rows' segments meanwhile.
@@ -243,12 +248,12 @@ __global__ __launch_bounds__(kSortThreads) void emb_scatter_kernel(KeySource src
                                                                    const uint32_t *__restrict__ hist, int64_t tiles,
                                                                    const uint32_t *__restrict__ totals,
                                                                    int32_t *__restrict__ out_key,
-                                                                   int32_t *__restrict__ out_pos, int32_t *hot_count) {
+                                                                   int32_t *__restrict__ out_pos, int32_t *__restrict__ hot_count) {
   __shared__ SortLds s;
   const int radix = 1 << dbits, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int64_t tile_base = (int64_t)blockIdx.x * kSortTile, left = n - tile_base;
   const int here = (int)(left < kSortTile ? left : kSortTile);
-  if (hot_count && blockIdx.x == 0 && threadIdx.x == 0) *hot_count = 0;
+  if (blockIdx.x == 0 && (int)threadIdx.x < kHotLists) hot_count[threadIdx.x * kHotStride] = 0;
   int32_t key[kKeysPerLane], pos[kKeysPerLane];
 #pragma unroll
   for (int r = 0; r < kKeysPerLane; ++r) {
@@ -327,7 +332,8 @@ struct SumArgs {
   void *out;
   int64_t ldo;
   float *partial;               // [2 * chunks][d], float32
-  int32_t *hot_count, *hot;     // parts (2 * chunk + which) that hot rows begin with, in any order
+  int32_t *hot_count, *hot;     // kHotLists lists of parts (2 * chunk + which) that hot rows begin with, in any order
+  int32_t hot_room;             // of one list
   int32_t teams;                // chunks of a workgroup
   unsigned chunk_groups;        // workgroups that stream; those behind them write the rows that no index names
 };
@@ -419,6 +425,11 @@ __device__ __forceinline__ void stream_rows(const SumArgs &a, const C &c, int32_
   done(now, sum);
 }
 
+__device__ __forceinline__ void list_hot(const SumArgs &a, int32_t part) {
+  const int list = blockIdx.x % kHotLists;
+  a.hot[(int64_t)list * a.hot_room + atomicAdd(a.hot_count + list * kHotStride, 1)] = part;
+}
+
 template <int DT, bool OUT_F32, int FIT>
 __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lanes_log) {
   typedef typename Elem<DT>::type T;
@@ -480,12 +491,12 @@ __global__ __launch_bounds__(kEmbThreads) void emb_sum_kernel(SumArgs a, int lan
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += sums[(t << lanes_log) + lane][i];
     if (c.any()) keep(partial, sum);
-    if (first.from == begin && lane == 0 && blockIdx.y == 0) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
+    if (first.from == begin && lane == 0 && blockIdx.y == 0) list_hot(a, 2 * chunk);
     return;
   }
   if (lane == 0 && blockIdx.y == 0) {
-    if (hot_first && first.from == begin) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk;
-    if (hot_last && last.from > begin) a.hot[atomicAdd(a.hot_count, 1)] = 2 * chunk + 1;
+    if (hot_first && first.from == begin) list_hot(a, 2 * chunk);
+    if (hot_last && last.from > begin) list_hot(a, 2 * chunk + 1);
   }
   // a light row that began in the chunk before is that chunk's, one that begins here is followed behind the end
   const int32_t from = !hot_first && first.from < begin ? first.to : begin, to = hot_last ? end : last.to;
@@ -510,10 +521,20 @@ __global__ __launch_bounds__(kWave *kFoldWaves) void emb_fold_kernel(SumArgs a, 
   __shared__ float lds[kFoldWaves][kFoldColumns];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int team = lane >> lanes_log, teams = kWave >> lanes_log;
-  const int32_t j = blockIdx.y * kFoldColumns + (lane & ((1 << lanes_log) - 1)) * 4, all = *a.count, hot = *a.hot_count;
+  const int32_t j = blockIdx.y * kFoldColumns + (lane & ((1 << lanes_log) - 1)) * 4, all = *a.count;
   const int live = a.d - j < 4 ? a.d - j : 4;
+  int32_t in_list[kHotLists], hot = 0;
+#pragma unroll
+  for (int l = 0; l < kHotLists; ++l) in_list[l] = a.hot_count[l * kHotStride];
+#pragma unroll
+  for (int l = 0; l < kHotLists; ++l) hot += in_list[l];
   for (int32_t h0 = blockIdx.x * teams; h0 < hot; h0 += gridDim.x * teams) {  // uniform in the workgroup
-    const int32_t part = a.hot[h0 + team < hot ? h0 + team : h0], chunk = part >> 1, which = part & 1, begin = chunk * a.span;
+    int32_t h = h0 + team < hot ? h0 + team : h0, list = 0;  // the h-th of all lists
+#pragma unroll
+    for (int l = 0; l < kHotLists - 1; ++l)
+      if (list == l && h >= in_list[l]) h -= in_list[l], ++list;
+    const int32_t part = a.hot[(int64_t)list * a.hot_room + h];
+    const int32_t chunk = part >> 1, which = part & 1, begin = chunk * a.span;
     const bool mine = h0 + team < hot && live > 0;
     const int32_t end = all - begin < a.span ? all : begin + a.span;
     const int32_t v = a.key[which ? end - 1 : begin];
@@ -623,10 +644,8 @@ __global__ __launch_bounds__(kSortThreads) void emb_small_kernel(KeySource src, 
     out_pos[i] = s.pos[i];
   }
   const int32_t all = segment_of(s.key, n, (int32_t)src.rows).from;
-  if (threadIdx.x == 0) {
-    *count = all;
-    *hot_count = 0;
-  }
+  if (threadIdx.x == 0) *count = all;
+  if ((int)threadIdx.x < kHotLists) hot_count[threadIdx.x * kHotStride] = 0;
   for (int32_t e = threadIdx.x; (e >> 1) * span < all; e += kSortThreads) {
     const int32_t begin = (e >> 1) * span, end = all - begin < span ? all : begin + span;
     const int32_t v = s.key[(e & 1) ? end - 1 : begin];
@@ -641,17 +660,20 @@ struct EmbPlan {
   int32_t span;
   size_t key[2], pos[2], hist, totals, segments, ends, counters, hot, partial, bytes;  // offsets into the workspace
 };
-static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
+static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d, size_t elem) {
   EmbPlan p = {};
   const int bits = bits_for((int32_t)(rows + 1));
   p.passes = (bits + kMaxDigit - 1) / kMaxDigit;
   p.dbits = (bits + p.passes - 1) / p.passes;
   p.tiles = ceil_div64(n, kSortTile);
   // About sqrt(n / 256): the longest chain of additions in a team and the longest list of partial rows grow alike.
-  // 232,965 x 128 float32 with popular indices takes 139 us in chunks of 64, 130 in chunks of 32 (as here) and of 16;
-  // 131,072 x 1024 bf16 143 us in chunks of 32 (as here) and 150 in chunks of 16.
+  // The gradient of 232,965 x 128 float32 with popular indices takes 69 us in chunks of 64 and of 32 (as here), 71 in chunks
+  // of 16; 131,072 x 1024 bf16 144 us in chunks of 32 (as here) and 156 in chunks of 16.
   p.span = 8;
   while (p.span < 512 && (int64_t)p.span * p.span * 256 < n) p.span *= 2;
+  // Rows of up to 128 bytes take 8 lanes or fewer: a quarter of that, or too few wavefronts run to hide their loads (1,000,000
+  // x 8 bf16 96 -> 73 us, 100,000 x 64 bf16 39 -> 31; rows of 240 bytes 116 -> 125, of 256 all of one row 128 -> 165).
+  if ((size_t)d * elem <= 128) p.span = p.span > 32 ? p.span / 4 : 8;
   p.chunks = ceil_div64(n, p.span);
   size_t at = 0;
   auto take = [&at](size_t bytes) {
@@ -664,8 +686,8 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d) {
   p.totals = take((size_t)kMaxRadix * 4);
   p.segments = take((size_t)rows * sizeof(Segment));
   p.ends = take(p.tiles <= 1 ? (size_t)p.chunks * 2 * sizeof(Segment) : 0);
-  p.counters = take(8);  // positions inside the table, hot rows
-  p.hot = take((size_t)p.chunks * 4);
+  p.counters = take((size_t)(1 + kHotLists) * kHotStride * 4);  // positions inside the table; hot rows of every list
+  p.hot = take(((size_t)p.chunks * 2 + 2 * kHotLists * kEmbThreads) * 4);
   p.partial = take((size_t)p.chunks * 2 * (size_t)d * 4);
   p.bytes = at;
   return p;
@@ -722,7 +744,8 @@ int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *byte
   using namespace cg;
   if (!bytes) CG_FAIL(CG_ERR_NULL, "cg_embedding_bwd_workspace: null pointer");
   CG_TRY(check_lookup("cg_embedding_bwd_workspace", n, rows, d));
-  *bytes = (int64_t)emb_plan(n, rows, d).bytes;
+  const size_t wide = emb_plan(n, rows, d, 4).bytes, narrow = emb_plan(n, rows, d, 2).bytes;
+  *bytes = (int64_t)(wide > narrow ? wide : narrow);
   return CG_OK;
 }
 
@@ -738,7 +761,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   if (!d_out || !d_work || (n > 0 && (!d_g || !d_idx))) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
   if (ldo < d || (n > 0 && ldg < d)) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
   if (d_out == d_g) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the input", who);
-  const EmbPlan p = emb_plan(n, rows, d);
+  const EmbPlan p = emb_plan(n, rows, d, elem_size(dtype));
   CG_TRY(check_work(who, d_work, work_bytes, (int64_t)p.bytes));
   hipStream_t s = (hipStream_t)stream;
   ProfScope prof("embedding_bwd", d, s);
@@ -751,7 +774,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   SumArgs a = {};
   a.g = d_g, a.ldg = ldg, a.count = counters, a.rows = rows, a.d = d, a.span = p.span, a.chunks = (int32_t)p.chunks;
   a.scale = scale, a.beta = beta, a.out = d_out, a.ldo = ldo, a.partial = (float *)(w + p.partial);
-  a.hot_count = counters + 1, a.hot = (int32_t *)(w + p.hot);
+  a.hot_count = counters + kHotStride, a.hot = (int32_t *)(w + p.hot);
   KeySource src = {{d_idx, idx64 != 0}, nullptr, nullptr, rows};
   const bool small = n > 0 && p.tiles <= 1 && (beta == 0.f || beta == 1.f);
   if (small) {
@@ -761,7 +784,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
     groups = 1 + (groups < 1024 ? groups : 1024);
 #define CG_CALL(OT)                                                                                                     \
   emb_small_kernel<<<(unsigned)groups, kSortThreads, 0, s>>>(src, (int32_t)n, p.passes, p.dbits, p.span, key[0], pos[0], ends, \
-                                                             counters, counters + 1, (Elem<OT>::type *)d_out, ldo, d)
+                                                             counters, counters + kHotStride, (Elem<OT>::type *)d_out, ldo, d)
     CG_BY_DTYPE(out_dtype, CG_CALL)
 #undef CG_CALL
     CG_LAUNCH_CHECK();
@@ -784,12 +807,12 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
       CG_LAUNCH_CHECK();
       if (direct) {
         emb_scatter_kernel<true><<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals,
-                                                                            key[to], pos[to], counters + 1);
+                                                                            key[to], pos[to], counters + kHotStride);
       } else {
         emb_scan_kernel<<<(unsigned)ceil_div64(radix, kEmbWaves), kEmbThreads, 0, s>>>(hist, p.tiles, radix, totals);
         CG_LAUNCH_CHECK();
         emb_scatter_kernel<false><<<(unsigned)p.tiles, kSortThreads, 0, s>>>(src, n, shift, p.dbits, hist, p.tiles, totals,
-                                                                             key[to], pos[to], counters + 1);
+                                                                             key[to], pos[to], counters + kHotStride);
       }
       CG_LAUNCH_CHECK();
       src.key = key[to], src.pos = pos[to];
@@ -804,6 +827,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   }
   const int per_chunk = dtype == CG_F32 ? 4 : 8, lanes_log = lanes_log2(d, per_chunk), teams = kEmbThreads >> lanes_log;
   a.teams = teams, a.chunk_groups = (unsigned)ceil_div64(p.chunks, teams);
+  a.hot_room = 2 * teams * (int32_t)ceil_div64(a.chunk_groups, kHotLists);  // every part of every chunk
   int64_t groups = small || beta == 1.f ? 0 : ceil_div64(rows, teams);
   if (groups > 256 * 16) groups = 256 * 16;
   groups += a.chunk_groups;
@@ -827,7 +851,8 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
 #undef CG_CALL
   CG_LAUNCH_CHECK();
   if (n <= p.span) return CG_OK;  // no row can be hot
-  const dim3 fold((unsigned)(p.chunks < 512 ? p.chunks : 512), (unsigned)ceil_div64(d, kFoldColumns));
+  const int64_t columns = ceil_div64(d, kFoldColumns), at_once = columns < 8 ? 512 / columns : 64;  // two workgroups a CU
+  const dim3 fold((unsigned)(p.chunks < at_once ? p.chunks : at_once), (unsigned)columns);
   int fold_lanes_log = lanes_log2(d, 4);
   if (fold_lanes_log > 6) fold_lanes_log = 6;
 #define CG_CALL(OT) emb_fold_kernel<OT><<<fold, kWave * kFoldWaves, 0, s>>>(a, fold_lanes_log)
