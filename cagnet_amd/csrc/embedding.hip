@@ -70,8 +70,8 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(const typena
 }
 
 // ---------------------------------------------------------------------------------------------
-// Stable radix sort of (key, position), digits of up to 10 bits: tables of up to a thousand rows take one pass, up to a million two.  A
-// workgroup of 16 wavefronts holds a tile of 4096 keys.  One tile is sorted in LDS by one launch; up to kDirectTiles
+// Stable radix sort of (key, position), digits of up to 10 bits: tables of up to a thousand rows take one pass, up to a
+// million two.  A workgroup of 16 wavefronts holds a tile of 4096 keys.  One tile is sorted in LDS by one launch; up to kDirectTiles
 // tiles take two launches a pass (count, scatter: every scatter workgroup adds the tiles' counts up itself, one row of
 // counts a tile); more tiles take a third that scans the counts, one wavefront a digit.
 // ---------------------------------------------------------------------------------------------
@@ -100,7 +100,8 @@ struct Segment {
 };
 
 // Hot rows are listed by one atomic each; kHotLists counters in cache lines of their own share them, because atomics on one
-// address follow each other at 25 ns (1,000,000 x 60 float32 popular indices: 126 us with one counter, 116 with eight; in chunks of 8 434 and 139).
+// address follow each other at 25 ns (1,000,000 x 60 float32 popular indices: 126 us with one counter, 116 with eight; in
+// chunks of 8 434 and 139).
 constexpr int kHotLists = 8, kHotStride = 64;
 
 // Counts of a tile's digits, at hist[digit * digit_step + tile * tile_step].  Workgroups behind the tiles clear the table

@@ -767,3 +767,28 @@ def test_results_are_contiguous_whatever_the_strides(cuda, n, d):
         same = [x, y2, ops.rms_norm_bwd(x, x, w, rstd)[0], r2, h2,
                 *ops.norm_residual_bwd(x, x, x, r2, w, w, rz, rr, gate=x)[:3]]
         assert all(torch.equal(a, b) for a, b in zip(outs, same))
+
+
+@pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])
+@pytest.mark.parametrize("t, d", [(torch.float32, 3), (torch.float32, 13), (torch.float32, 64), (torch.float32, 70),
+                                  (torch.bfloat16, 5), (torch.bfloat16, 55), (torch.float16, 261), (torch.float16, 600)])
+def test_embedding_many_hot_rows(cuda, t, d, beta):
+    # every table row but the last ten has about 100 positions, row 7 a third of all; the first index is padding
+    from cagnet_amd import ops
+
+    gen = torch.Generator().manual_seed(d)
+    n, rows = 60_000, 410
+    idx = torch.randint(0, rows - 10, (n,), generator=gen)
+    idx[torch.rand(n, generator=gen) < 1 / 3] = 7
+    idx[0] = rows
+    g, old = torch.randn(n, d, generator=gen).to(t), torch.randn(rows, d, generator=gen).to(t)
+    out = old.to(cuda)
+    ops.embedding_bwd(g.to(cuda), idx.to(cuda), rows, 0.5, out=out, beta=beta)
+    want, size = torch.zeros(rows + 1, d, dtype=torch.float64), torch.zeros(rows + 1, d, dtype=torch.float64)
+    want.index_add_(0, idx, g.double()), size.index_add_(0, idx, g.double().abs())
+    want, size = (0.5 * want + beta * torch.cat([old, old[:1]]).double())[:rows], (0.5 * size)[:rows] + beta * old.double().abs()
+    # a sum of k terms in float32 in any order is off by (k - 1) 2^-24 of their size at most; + scale, beta and the sum
+    count = torch.bincount(idx, minlength=rows + 1)[:rows, None].double()
+    bound = (count + 4) * 2.0**-24 * size
+    bound = bound + (torch.finfo(t).eps / 2) * (want.abs() + bound) + torch.finfo(t).smallest_normal
+    assert bool(((out.cpu().double() - want).abs() <= bound).all())
