@@ -20,7 +20,6 @@ from typing import List, Optional, Sequence, Union
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import ops
 from .ops import CsrMatrix
@@ -391,21 +390,48 @@ class LogSoftmaxNLLLoss(torch.autograd.Function):
 # deeper than the reference's two layers (which have no counterpart of these):
 #   x = dropout(embedding(table, ids), p, rng_next(state));  h = rms_norm(x, w_0)
 #   z = GCNFunc.apply(h, W_k, ...);  x, h = norm_residual(z, x, w_post, w_pre, gate, scale)      for every layer k
-# First derivatives only.
+# First derivatives only: a second one raises.
 # ------------------------------------------------------------------------------------------------
 rng_state, rng_next = ops.rng_state, ops.rng_next
 
 
-def _first_order(backward):
-    """A backward pass without a gradient of its own.  The engine turns recording off unless create_graph asks for it;
-    only then the wrapper that refuses second derivatives is needed (a step of a few rows is bound by the host)."""
-    guarded = once_differentiable(backward)
+class _FirstOnly(torch.autograd.Function):
+    """Gradients (behind the first `count` tensors) as they are, as functions of those first ones that cannot be
+    differentiated: an engine that is asked for the derivative by any of them comes through here."""
 
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    @staticmethod
+    def forward(ctx, count, *tensors):
+        return tensors[count:]
 
-    return run
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("first derivatives only: this gradient is once_differentiable")
+
+
+def _first_order(linear: bool):
+    """Marks a backward pass without a gradient of its own.  The engine turns recording off unless create_graph asks for
+    it; only then the results are made to refuse a second derivative (a step of a few rows is bound by the host).
+    `linear`: the gradient depends on nothing but the incoming one, so that where that is a constant so is the result, and
+    its second derivative is zero.  Everywhere else it depends on what the forward pass saved too, also where the incoming
+    gradient is a constant (that of a sum), and a result without a node would drop that dependence without a word."""
+
+    def mark(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                outs = backward(ctx, *grads)
+            of = [t for t in (grads if linear else (*grads, *ctx.saved_tensors)) if t is not None and t.requires_grad]
+            given = [o for o in outs if o is not None]
+            if not of or not given:
+                return outs
+            marked = iter(_FirstOnly.apply(len(of), *of, *given))
+            return tuple(None if o is None else next(marked) for o in outs)
+
+        return run
+
+    return mark
 
 
 class Dropout(torch.autograd.Function):
@@ -418,7 +444,7 @@ class Dropout(torch.autograd.Function):
         return ops.dropout_fwd(x, p, rng)
 
     @staticmethod
-    @_first_order
+    @_first_order(linear=True)
     def backward(ctx, g):
         return ops.dropout_bwd(g, ctx.p, ctx.saved_tensors[0] if ctx.has_rng else None), None, None
 
@@ -441,7 +467,7 @@ class Embedding(torch.autograd.Function):
         return out if idx.dim() == 1 else out.view(*idx.shape, table.shape[1])
 
     @staticmethod
-    @_first_order
+    @_first_order(linear=True)
     def backward(ctx, g):
         (flat,) = ctx.saved_tensors
         g = g if g.dim() == 2 else g.reshape(-1, ctx.width)
@@ -463,7 +489,7 @@ class RmsNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_first_order
+    @_first_order(linear=False)
     def backward(ctx, g):
         x, rstd, *weight = ctx.saved_tensors
         dx, dw = ops.rms_norm_bwd(g, x, weight[0] if weight else None, rstd)
@@ -489,7 +515,7 @@ class NormResidual(torch.autograd.Function):
         return r, h
 
     @staticmethod
-    @_first_order
+    @_first_order(linear=False)
     def backward(ctx, dr, dh):
         if dr is None and dh is None:
             return (None,) * 10
