@@ -174,7 +174,8 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
       }
       continue;
     }
-    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid((float)gate[0]) : 1.f;
+    float row_slope = 0.f;
+    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid((float)gate[0], row_slope) : 1.f;
     auto through = [&](float (&D)[V], float (&zh)[V], float (&f)[V], bool outputs) {  // f: gradient of the normalised z
       float w[V], t[V], sig[V];
       into(D);
@@ -193,8 +194,9 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
         c.floats(c.load(gate), t);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          sig[i] = sigmoid(t[i]);
-          t[i] = f[i] * zh[i] * (sig[i] * (1.f - sig[i]));
+          float slope;
+          sig[i] = sigmoid(t[i], slope);
+          t[i] = f[i] * zh[i] * slope;
         }
         if (outputs) c.write((T *)a.dgate + row * a.lddgate, t);
       }
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
       s += c.dot(f, zh);
     }
     s = row_sum<kWave, true>(s, slots, turn);
-    if (a.gate_kind == CG_GATE_ROW && threadIdx.x == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));
+    if (a.gate_kind == CG_GATE_ROW && threadIdx.x == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * row_slope);
     const float mean_z = s / (float)a.d;
     for (int32_t j = start; j < a.d; j += step) {
       float D[V], zh[V], f[V];

@@ -40,10 +40,18 @@ __device__ __forceinline__ void fold_columns(float (&acc)[K][C::V], const C (&c)
 
 // The bound on registers, where 8 elements of 16 bits a lane miss it by a few: four wavefronts a SIMD for rows of whole
 // chunks (2,343,750 x 64 bf16: 420 us without, 353 with), three for others, which would have to spill for the fourth
-// (3,658,536 x 41 bf16 with row gates and dropout: 872 us with four, 705 with three).
+// (3,658,536 x 41 bf16 with row gates and dropout: 872 us with four, 705 with three).  In float32 the
+// bounds only keep the compiler from taking a register or two too many for them (nothing is spilled).
+template <int DT, int K, bool WHOLE, int FIT, bool RESIDUAL>
+constexpr int bwd_waves() {
+  if (!RESIDUAL || WHOLE) return 1;
+  if (DT == CG_F32) return K == 1 ? 5 : FIT != kWholeChunks ? 1 : K == 2 ? 4 : 2;
+  return K > 1 ? 1 : FIT == kPartChunk ? 3 : 4;
+}
+
 template <int DT, int LANES, int K, bool WHOLE, int FIT, bool RESIDUAL>
 __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads,
-                             !RESIDUAL || DT == CG_F32 || K > 1 ? 1 : FIT == kPartChunk ? 3 : 4) void norm_bwd_kernel(NormArgs a) {
+                             (bwd_waves<DT, K, WHOLE, FIT, RESIDUAL>())) void norm_bwd_kernel(NormArgs a) {
   typedef typename Elem<DT>::type T;
   typedef Span<T, FIT> C;
   constexpr int V = C::V, TEAMS = WHOLE ? 1 : kNormThreads / LANES;
@@ -160,7 +168,8 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads,
         for (int i = 0; i < V; ++i) D[k][i] += g[i];
       }
     }
-    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid(row_gate) : 1.f;
+    float row_slope = 0.f;
+    const float row_sig = a.gate_kind == CG_GATE_ROW ? sigmoid(row_gate, row_slope) : 1.f;
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -175,9 +184,10 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads,
         c[k].floats(rg[k], g);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float sig = sigmoid(g[i]), e = D[k][i] * wz[k][i];
+          float slope;
+          const float sig = sigmoid(g[i], slope), e = D[k][i] * wz[k][i];
           q[k][i] += D[k][i] * sig * zh[k][i];
-          g[i] = e * zh[k][i] * (sig * (1.f - sig));
+          g[i] = e * zh[k][i] * slope;
           D[k][i] = e * sig;
         }
         c[k].write((T *)a.dgate + row * a.lddgate, g);
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(WHOLE ? kWave * kNormMaxWaves : kNormThreads,
       s += c[k].dot(D[k], zh[k]);
     }
     s = row_sum<LANES, WHOLE>(s, slots, turn);
-    if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * (row_sig * (1.f - row_sig)));
+    if (a.gate_kind == CG_GATE_ROW && lane == 0) ((T *)a.dgate)[row * a.lddgate] = rounded<T>(s * row_slope);
     const float m = s * inv_d, rho_s = rho_z * row_sig;
 #pragma unroll
     for (int k = 0; k < K; ++k) {

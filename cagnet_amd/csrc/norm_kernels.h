@@ -81,5 +81,13 @@ __device__ __forceinline__ float row_sum(float v, NormSlots &slots, int &turn) {
 __device__ __forceinline__ float sigmoid(float a) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.44269504f));
 }
+// The same with its derivative s (1 - s).  With s rounded to 24 bits, 1 - s has lost its leading digits where s is near 1
+// (at a = 10 about a thousandth of it is wrong, from 17 on it is 0); there e^-a s is the same number without a difference.
+// Up to a half 1 - s is exact to a rounding, and e^-a can be infinite.
+__device__ __forceinline__ float sigmoid(float a, float &slope) {
+  const float e = __builtin_amdgcn_exp2f(a * -1.44269504f), s = __builtin_amdgcn_rcpf(1.f + e);
+  slope = s * (s > 0.5f ? e * s : 1.f - s);
+  return s;
+}
 
 }  // namespace cg

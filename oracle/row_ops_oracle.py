@@ -110,7 +110,8 @@ def norm_residual_grad(dr, dh, z, r, w_post, w_pre, rho_z, rho_r, gate, scale, a
     out["dscale"] = (alpha * w_post * q, abs(alpha) * w_post.abs() * q_mag)
     c = alpha * scale * w_post
     if gate is not None:
-        dg, dg_mag = D * c * zh * sig * (1 - sig), M * c.abs() * zh.abs() * sig  # 1 - sig cancels: its terms are <= 1
+        slope = sig * torch.sigmoid(-gate.double())  # 1 - sig would cancel
+        dg, dg_mag = D * c * zh * slope, M * c.abs() * zh.abs() * slope
         if gate.shape[1] == 1 and d > 1:
             dg, dg_mag = dg.sum(dim=1, keepdim=True), dg_mag.sum(dim=1, keepdim=True)
         out["dgate"] = (dg, dg_mag)
