@@ -635,6 +635,7 @@ def log_softmax_nll_bwd(logp: torch.Tensor, y: torch.Tensor, mask: Optional[torc
 # Temporary memory comes from torch's allocator, so that a captured graph owns its own.
 # ------------------------------------------------------------------------------------------------
 _ROW_DTYPES = {torch.float32: _lib.CG_F32, torch.bfloat16: _lib.CG_BF16, torch.float16: _lib.CG_F16}
+_MOST_COLUMNS = (1 << 31) - 1  # the C ABI counts columns in 32 bits, and ctypes would drop the bits above without a word
 
 
 # torch.cuda.current_device() and current_stream() build Python objects; a call on a few thousand rows is bound by the
@@ -677,6 +678,8 @@ def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> Tu
     rows, cols = shape
     if cols == 0:
         raise ValueError(f"{name}: rows of no elements")
+    if cols > _MOST_COLUMNS:
+        raise ValueError(f"{name}: rows of {cols} elements (at most {_MOST_COLUMNS})")
     ld, step = t.stride()
     if (cols > 1 and step != 1) or (rows > 1 and ld < cols):
         t = t.contiguous()
