@@ -534,12 +534,20 @@ def norm_residual(z: torch.Tensor, x: torch.Tensor, w_post: Optional[torch.Tenso
     return NormResidual.apply(z, x, w_post, w_pre, gate, scale, alpha, p, rng, eps)
 
 
+def _rank_masks(snapshot: torch.Tensor, rank: int) -> torch.Tensor:
+    """A mask goes by the row's number within its block, which every rank counts from zero: with one seed all ranks would
+    drop the same places of their blocks.  So rank r takes the masks of the offsets from r 2^48 on, which no other reaches."""
+    if rank:
+        snapshot[1:].add_(((rank + (1 << 15)) % (1 << 16) - (1 << 15)) << 48)
+    return snapshot
+
+
 def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank=0, size=1, group=None,
           dropout_p: float = 0.0, rng: Optional[torch.Tensor] = None):
     """One epoch, gcn_distr.py:341-366.  `data` needs `.y` and `.train_mask`; `group` is None for a
     whole graph on one GPU, or a pair (layer-1 ResidentBlocks, layer-2 ResidentBlocks).  dropout_p > 0 drops
     hidden activations between the two layers (the reference has none); `rng` is then the generator state
-    (`rng_state`), which every epoch steps once."""
+    (`rng_state`), which every epoch steps once.  Ranks may share one seed: each draws masks of its own."""
     g1, g2 = group if isinstance(group, (tuple, list)) else (group, group)
     if not 0.0 <= dropout_p <= 1.0:
         raise ValueError(f"train: dropout probability {dropout_p} outside [0, 1]")
@@ -547,7 +555,7 @@ def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, 
         raise ValueError("train: dropout_p > 0 needs a generator state (rng)")
     outputs = GCNFunc.apply(inputs, weight1, adj_matrix, am_partitions, rank, size, g1, F.relu)
     if dropout_p > 0.0:
-        outputs = dropout(outputs, dropout_p, rng_next(rng))
+        outputs = dropout(outputs, dropout_p, _rank_masks(rng_next(rng), rank))
     fuse = fused_loss and activations
     outputs = GCNFunc.apply(outputs, weight2, adj_matrix, am_partitions, rank, size, g2, None if fuse else F.log_softmax)
 
