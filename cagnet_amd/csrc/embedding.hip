@@ -695,7 +695,7 @@ static EmbPlan emb_plan(int64_t n, int64_t rows, int32_t d, size_t elem) {
 }
 
 static int check_lookup(const char *who, int64_t n, int64_t rows, int32_t d) {
-  if (n < 0 || rows <= 0 || d <= 0)
+  if (n < 0 || rows < 0 || (rows == 0 && n > 0) || d <= 0)
     CG_FAIL(CG_ERR_SIZE, "%s: n=%lld indices into rows=%lld of d=%d elements", who, (long long)n, (long long)rows, d);
   if (d > (1 << 23)) CG_FAIL(CG_ERR_OVERFLOW, "%s: rows of d=%d elements (at most 2^23)", who, d);
   if (n > 0x7ff00000LL || rows > 0x7ffffffdLL)
@@ -745,6 +745,8 @@ int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *byte
   using namespace cg;
   if (!bytes) CG_FAIL(CG_ERR_NULL, "cg_embedding_bwd_workspace: null pointer");
   CG_TRY(check_lookup("cg_embedding_bwd_workspace", n, rows, d));
+  *bytes = 0;
+  if (rows == 0) return CG_OK;
   const size_t wide = emb_plan(n, rows, d, 4).bytes, narrow = emb_plan(n, rows, d, 2).bytes;
   *bytes = (int64_t)(wide > narrow ? wide : narrow);
   return CG_OK;
@@ -759,6 +761,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
   if (out_dtype != dtype && out_dtype != CG_F32)
     CG_FAIL(CG_ERR_UNSUPPORTED, "%s: output dtype %d for gradients of dtype %d (the same or CG_F32)", who, out_dtype, dtype);
   CG_TRY(check_lookup(who, n, rows, d));
+  if (rows == 0) return CG_OK;
   if (!d_out || !d_work || (n > 0 && (!d_g || !d_idx))) CG_FAIL(CG_ERR_NULL, "%s: null pointer", who);
   if (ldo < d || (n > 0 && ldg < d)) CG_FAIL(CG_ERR_SIZE, "%s: leading dimension smaller than d", who);
   if (d_out == d_g) CG_FAIL(CG_ERR_ALIAS, "%s: the output may not be the input", who);

@@ -311,7 +311,8 @@ int cg_dropout(const void *d_x, int64_t ldx, void *d_out, int64_t ldo, int64_t n
                const int64_t *d_rng, cg_stream_t stream);
 
 /* out_i = scale * table[idx_i] for n indices (int32, or int64 when idx64 != 0) into `rows` rows; an
- * index outside [0, rows) gives a row of zeros (padding).  No counterpart in the reference. */
+ * index outside [0, rows) gives a row of zeros (padding).  The table may be empty when n == 0.  No
+ * counterpart in the reference. */
 int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void *d_idx, int idx64, int64_t n, int32_t d,
                      int dtype, float scale, void *d_out, int64_t ldo, cg_stream_t stream);
 /* Its gradient, out_v = scale * sum_{i: idx_i = v} g_i + beta * out_v for every table row v (rows no index
