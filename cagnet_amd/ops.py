@@ -639,9 +639,10 @@ _MOST_COLUMNS = (1 << 31) - 1  # the C ABI counts columns in 32 bits, and ctypes
 
 
 # torch.cuda.current_device() and current_stream() build Python objects; a call on a few thousand rows is bound by the
-# host (about 3 us of kernel against 10 us of Python), so the raw handles are taken from underneath them.
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# host (about 3 us of kernel against 10 us of Python), so the raw handles are taken from underneath them, where this
+# torch has these (they are not part of its public interface).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _run(device: torch.device, where: str, fn, *args) -> None:
