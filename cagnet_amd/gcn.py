@@ -579,6 +579,17 @@ def train(inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, 
 train.last_loss = None
 
 
+def _recorded_elsewhere(leaf: torch.Tensor) -> bool:
+    """Whether an autograd graph that ends in `leaf` is alive.  All graphs of a leaf end in one node, which lives as long
+    as any of them: a mark left on the node of a graph of our own is found again only if another one holds it."""
+    if not (leaf.requires_grad and leaf.is_leaf):
+        return False
+    node = torch.autograd.graph.get_gradient_edge(leaf).node
+    node.metadata["cagnet_amd"] = True
+    del node
+    return "cagnet_amd" in torch.autograd.graph.get_gradient_edge(leaf).node.metadata
+
+
 class GraphedTrain:
     """`train` captured once into a HIP graph and replayed: one launch per epoch instead of some
     forty.  On graphs of a few thousand vertices an epoch is bound by launches and host work, not
@@ -592,6 +603,9 @@ class GraphedTrain:
     replays it.  Every tensor the epoch reads (`inputs`, the weights, `data.y`, `data.train_mask`)
     is read from the same memory on every replay: update them in place.  Optimizers that keep
     scalars on the host must be built for capture (`torch.optim.Adam(..., capturable=True)`).
+    No autograd graph of `inputs` or the weights may be alive (drop or detach what was computed from them): the
+    node that adds up a leaf's gradient belongs to the stream it was made on, and capturing a backward pass
+    into it from another stream ends the process.  The constructor refuses such a call.
     With `dropout_p` the generator state `rng` is read and stepped on the device: every replay draws a new mask.
 
     The graph replays with the addresses of the library's scratch buffers of its stream and of the
@@ -605,6 +619,10 @@ class GraphedTrain:
                  group=None, warmup: int = 3, dropout_p: float = 0.0, rng: Optional[torch.Tensor] = None):
         if warmup < 1:
             raise ValueError("at least one warm-up epoch is needed: it builds the schedules and grows the scratch")
+        for name, leaf in (("inputs", inputs), ("weight1", weight1), ("weight2", weight2)):
+            if _recorded_elsewhere(leaf):
+                raise RuntimeError(f"{name}: outputs computed from it earlier are still alive with their autograd graph; "
+                                   "drop or detach them before the epoch is captured")
         args = (inputs, weight1, weight2, adj_matrix, am_partitions, optimizer, data, rank, size, group, dropout_p, rng)
         self.stream = torch.cuda.Stream(device=weight1.device)
         self.stream.wait_stream(torch.cuda.current_stream(weight1.device))
