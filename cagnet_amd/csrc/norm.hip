@@ -234,8 +234,10 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_rows_kernel(NormArgs a)
 }
 
 // dw_post = alpha scale q, dscale = alpha w_post q, dw_pre: the slices of `partial` added up.  One workgroup per 16
-// columns; 64 threads share a column, each adds every 64th slice in order, then the 64 sums are added in order.
+// columns; 64 threads share a column, each adds every 64th slice in order, then the 64 sums are added in order.  A launch
+// holds fewer than 2^32 threads, so that the workgroups of very long rows take more than one stretch of columns each.
 constexpr int kFoldCols = 16, kFoldTeams = 64;
+constexpr int64_t kFoldGroups = 1 << 20;
 
 template <int DT, bool RESIDUAL>
 __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kernel(NormArgs a, int32_t slices, void *dw_post,
@@ -243,30 +245,34 @@ __global__ __launch_bounds__(kFoldCols *kFoldTeams) void norm_weight_grads_kerne
   typedef typename Elem<DT>::type T;
   __shared__ float sq[kFoldTeams][kFoldCols + 1], sp[kFoldTeams][kFoldCols + 1];
   const int col = threadIdx.x % kFoldCols, team = threadIdx.x / kFoldCols;
-  const int32_t j = blockIdx.x * kFoldCols + col;
   const int64_t step = (int64_t)(RESIDUAL ? 2 : 1) * a.d;
-  float q = 0.f, p = 0.f;
-  if (j < a.d) {
+  for (int32_t j0 = blockIdx.x * kFoldCols; j0 < a.d; j0 += gridDim.x * kFoldCols) {  // once for rows of up to 2^24 columns
+    const int32_t j = j0 + col;
+    float q = 0.f, p = 0.f;
+    if (j < a.d) {
 #pragma unroll 8
-    for (int32_t k = team; k < slices; k += kFoldTeams) {
-      const float *at = a.partial + k * step + j;
-      q += at[0];
-      if (RESIDUAL) p += at[a.d];
+      for (int32_t k = team; k < slices; k += kFoldTeams) {
+        const float *at = a.partial + k * step + j;
+        q += at[0];
+        if (RESIDUAL) p += at[a.d];
+      }
     }
-  }
-  sq[team][col] = q;
-  if (RESIDUAL) sp[team][col] = p;
-  __syncthreads();
-  if (team != 0 || j >= a.d) return;
-  q = p = 0.f;
+    sq[team][col] = q;
+    if (RESIDUAL) sp[team][col] = p;
+    __syncthreads();
+    if (team == 0 && j < a.d) {
+      q = p = 0.f;
 #pragma unroll 8
-  for (int t = 0; t < kFoldTeams; ++t) {
-    q += sq[t][col];
-    if (RESIDUAL) p += sp[t][col];
+      for (int t = 0; t < kFoldTeams; ++t) {
+        q += sq[t][col];
+        if (RESIDUAL) p += sp[t][col];
+      }
+      if (dw_post) weight_put<T>(dw_post, a.w_f32, j, a.alpha * weight_at<T>(a.scale, a.w_f32, j) * q);
+      if (dscale) weight_put<T>(dscale, a.w_f32, j, a.alpha * weight_at<T>(a.w_post, a.w_f32, j) * q);
+      if (dw_pre) weight_put<T>(dw_pre, a.w_f32, j, p);
+    }
+    __syncthreads();  // the sums have been read
   }
-  if (dw_post) weight_put<T>(dw_post, a.w_f32, j, a.alpha * weight_at<T>(a.scale, a.w_f32, j) * q);
-  if (dscale) weight_put<T>(dscale, a.w_f32, j, a.alpha * weight_at<T>(a.w_post, a.w_f32, j) * q);
-  if (dw_pre) weight_put<T>(dw_pre, a.w_f32, j, p);
 }
 
 // ---- host side ------------------------------------------------------------------------------------
@@ -331,7 +337,8 @@ static int norm_bwd(const NormArgs &a, int dtype, void *dw_post, void *dw_pre, v
     CG_LAUNCH_CHECK();
   }
   if (dw_post || dw_pre || dscale) {
-    const unsigned cols = (unsigned)ceil_div64(a.d, kFoldCols);
+    const int64_t stretches = ceil_div64(a.d, kFoldCols);
+    const unsigned cols = (unsigned)(stretches < kFoldGroups ? stretches : kFoldGroups);
 #define CG_CALL(DT)                                                                                            \
   norm_weight_grads_kernel<DT, RESIDUAL><<<cols, kFoldCols * kFoldTeams, 0, s>>>(a, (int32_t)groups, dw_post, \
                                                                                  dw_pre, dscale)
