@@ -117,7 +117,7 @@ static int go(const NormArgs &a, bool residual, const NormShape &sh, int64_t gro
 }
 
 template <int DT>
-static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_t s) {
+static int go_shape(const NormArgs &a, bool residual, hipStream_t s) {
   constexpr int MOST = DT == CG_F32 ? 4 : 2;  // chunks of 16 elements
   const NormShape sh = norm_shape(a.d, DT, false);
   // Few rows a wave: the loads of a wave's next row would wait for the stores of the row before (they are counted
@@ -127,7 +127,7 @@ static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_
   const bool costly = residual && DT != CG_F32 && !sh.whole && a.d % 8 != 0;
   const int64_t want = ceil_div64(a.n, norm_rows_at_once(sh));
   const int64_t most = sh.whole ? 256 * 256 / (sh.threads / kWave) : costly ? 256 * 32 : 256 * 128;
-  groups = want < most ? want : most;
+  const int64_t groups = want < most ? want : most;
   if (sh.whole) return go<DT, kWave, MOST, true>(a, residual, sh, groups, s);
   if (sh.lanes == 4) return go<DT, 4, 1, false>(a, residual, sh, groups, s);
   if (sh.lanes == 8) return go<DT, 8, 1, false>(a, residual, sh, groups, s);
@@ -140,9 +140,9 @@ static int go_shape(const NormArgs &a, bool residual, int64_t groups, hipStream_
 }
 
 int launch_norm_fwd(const NormArgs &a, bool residual, int dtype, hipStream_t s) {
-  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, 0, s);
-  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, 0, s);
-  return go_shape<CG_F16>(a, residual, 0, s);
+  if (dtype == CG_F32) return go_shape<CG_F32>(a, residual, s);
+  if (dtype == CG_BF16) return go_shape<CG_BF16>(a, residual, s);
+  return go_shape<CG_F16>(a, residual, s);
 }
 
 }  // namespace cg

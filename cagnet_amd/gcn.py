@@ -390,6 +390,8 @@ class LogSoftmaxNLLLoss(torch.autograd.Function):
 # deeper than the reference's two layers (which have no counterpart of these):
 #   x = dropout(embedding(table, ids), p, rng_next(state));  h = rms_norm(x, w_0)
 #   z = GCNFunc.apply(h, W_k, ...);  x, h = norm_residual(z, x, w_post, w_pre, gate, scale)      for every layer k
+# Activations are [n, d]; a lookup of indices of another shape is flattened before it enters the other operators.  GCNFunc
+# and the losses take float32 only: 16-bit activations have to be cast on the way in and out of them.
 # First derivatives only: a second one raises.
 # ------------------------------------------------------------------------------------------------
 rng_state, rng_next = ops.rng_state, ops.rng_next
@@ -450,7 +452,8 @@ class Dropout(torch.autograd.Function):
 
 
 def dropout(x: torch.Tensor, p: float, rng: Optional[torch.Tensor]) -> torch.Tensor:
-    """x / (1 - p) where kept, 0 elsewhere; `rng` is a snapshot from `rng_next`, one for every dropout of a step.
+    """x [n, d] / (1 - p) where kept, 0 elsewhere; `rng` is a snapshot from `rng_next`, one for every dropout of a step.
+    The mask goes by row and column: where ranks hold blocks of one matrix, each needs a seed, or a range of offsets, of its own.
     A `rng` that is stepped or written before the gradient ran is refused by autograd's version check."""
     return Dropout.apply(x, p, rng)
 
@@ -497,7 +500,7 @@ class RmsNorm(torch.autograd.Function):
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6) -> torch.Tensor:
-    """x / sqrt(mean of x^2 over the row + eps) * weight."""
+    """x [n, d] / sqrt(mean of x^2 over the row + eps) * weight."""
     return RmsNorm.apply(x, weight, eps)
 
 

@@ -286,7 +286,8 @@ int cg_log_softmax_nll_fwd(const float *d_z, int64_t ldz, const int64_t *d_y, co
  * them (no counterpart; its layers end in F.relu / F.log_softmax, gcn_distr.py:284-294).
  * Arithmetic is float32 whatever the type, rounded once at each store.  Weight vectors ([d], NULL =
  * ones) and their gradients are float32 or have the activations' type (`wdtype`, one for all).
- * n rows (at most 2^32 - 1) of d columns (norms: at most 2^30); n == 0 is legal (weight gradients are then zero).
+ * n rows (at most 2^32 - 1) of d columns (norms: at most 2^30; embedding: limits of its own, below); n == 0
+ * is legal (weight gradients are then zero).
  * Outputs may not overlap inputs (cg_dropout may run in place).  Nothing is allocated and nothing is
  * read back: the gradients that need temporary memory take it from the caller (`d_work`, at least the
  * size the matching *_workspace function names, 16-byte aligned), so that every call can be captured
@@ -311,15 +312,15 @@ int cg_dropout(const void *d_x, int64_t ldx, void *d_out, int64_t ldo, int64_t n
                const int64_t *d_rng, cg_stream_t stream);
 
 /* out_i = scale * table[idx_i] for n indices (int32, or int64 when idx64 != 0) into `rows` rows; an
- * index outside [0, rows) gives a row of zeros (padding).  The table may be empty when n == 0.  No
- * counterpart in the reference. */
+ * index outside [0, rows) gives a row of zeros (padding).  The table may be empty when n == 0.
+ * CG_ERR_OVERFLOW from 2^31 - 2^20 indices, 2^31 - 2 table rows or 2^23 + 1 columns on.  No counterpart
+ * in the reference. */
 int cg_embedding_fwd(const void *d_table, int64_t ldt, int64_t rows, const void *d_idx, int idx64, int64_t n, int32_t d,
                      int dtype, float scale, void *d_out, int64_t ldo, cg_stream_t stream);
 /* Its gradient, out_v = scale * sum_{i: idx_i = v} g_i + beta * out_v for every table row v (rows no index
  * names get beta * out_v, and are neither read nor written when beta == 1; beta == 0 never reads out).
  * out has the type of g or is float32 (`out_dtype`).  Indices outside the table add to nothing.  The
- * additions of a row run in a fixed order that depends on the indices alone.  CG_ERR_OVERFLOW from
- * 2^31 - 2^20 indices, 2^31 - 2 table rows or 2^23 + 1 columns on. */
+ * additions of a row run in a fixed order that depends on the indices alone.  The limits of the lookup. */
 int cg_embedding_bwd_workspace(int64_t n, int64_t rows, int32_t d, int64_t *bytes);
 int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64, int64_t n, int64_t rows, int32_t d,
                      int dtype, int out_dtype, float scale, float beta, void *d_out, int64_t ldo, void *d_work,
@@ -327,6 +328,7 @@ int cg_embedding_bwd(const void *d_g, int64_t ldg, const void *d_idx, int idx64,
 
 /* y = x rstd w with rstd = 1 / sqrt(mean over the row of x^2 + eps), eps > 0; rstd is written for the
  * gradient dx = rstd (g w - x rstd mean(g w x rstd)), dw = sum over rows of g x rstd (d_dw nullable).
+ * The sum of squares is float32: a row that takes it beyond 3.4e38 (elements of 1e19) has rstd 0.
  * No counterpart in the reference. */
 int cg_rms_norm_fwd(const void *d_x, int64_t ldx, const void *d_w, int wdtype, void *d_y, int64_t ldy, float *d_rstd,
                     int64_t n, int32_t d, int dtype, float eps, cg_stream_t stream);

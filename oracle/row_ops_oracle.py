@@ -1,7 +1,8 @@
 """CPU restatement of the row-wise training operators in 64 bits (test infrastructure: the product never imports it).
 
-The generator is Philox 4x32 (Salmon, Moraes, Dror, Shaw 2011) on numpy's unsigned 64-bit integers; the operators are
-written forward only, and their gradients come from torch's automatic differentiation in float64.
+The generator is Philox 4x32 (Salmon, Moraes, Dror, Shaw 2011) on numpy's unsigned 64-bit integers.  The gradients are
+closed forms of given row statistics, with the magnitudes of the terms they sum for the tests' bounds; they are pinned to
+torch's automatic differentiation of the forward functions in float64, and those to differences.
 """
 from __future__ import annotations
 
@@ -33,15 +34,6 @@ def keep_mask(seed: int, offset: int, n: int, d: int, p: float, row0: int = 0) -
     words = np.stack(np.broadcast_arrays(*words), axis=2).reshape(n, -1)[:, :d]
     threshold = int(np.floor(p * 4294967296.0 + 0.5))
     return torch.from_numpy(np.ascontiguousarray(words >= np.uint64(threshold)))
-
-
-def dropout(x: torch.Tensor, p: float, seed: int, offset: int) -> torch.Tensor:
-    """In 64 bits; dropped elements are zero whatever x holds there."""
-    if p == 0.0:
-        return x.double()
-    keep = keep_mask(seed, offset, x.shape[0], x.shape[1], p)
-    return torch.where(keep, x.double() / (1.0 - p) if p < 1.0 else torch.zeros_like(x, dtype=torch.float64),
-                       torch.zeros((), dtype=torch.float64))
 
 
 def embedding(table: torch.Tensor, idx: torch.Tensor, scale: float) -> torch.Tensor:
